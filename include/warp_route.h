@@ -79,6 +79,8 @@ typedef enum wr_status {
   WR_EINVAL_SCRATCH = 12,     /* the problem needs more workspace than the
                                  allocation-free entry point's fixed scratch
                                  (WR_NOALLOC_SCRATCH_BYTES)                   */
+  WR_EINVAL_ALIGN = 13,       /* a pointer of a dense FFN or int8 call
+                                 (wr_ffn.h) is not 16-byte aligned            */
   WR_EHIP = 100               /* a HIP runtime call failed                     */
 } wr_status;
 

@@ -1,7 +1,7 @@
 """In-tree build of the gfx950 MoE library and its torch extension.
 
   libwarp_route_hip.so  hipcc --offload-arch=gfx950, from csrc/*.hip; exports
-                        exactly the C-ABI of include/warp_route.h
+                        exactly the C-ABI of include/warp_route.h and include/wr_ffn.h
   _C.<ext-suffix>.so    the pybind11/torch module warp_route._C, compiled
                         from csrc/bindings.cpp with the host compiler and
                         linked against libwarp_route_hip.so (rpath $ORIGIN)
@@ -47,7 +47,8 @@ HIP_FLAGS = [
     "-Wall", "-Wno-unused-function",
     *shlex.split(os.environ.get("WR_HIPCC_FLAGS", "")),
 ]
-HIP_SOURCES = ["wr_api.hip", "wr_kernels.hip", "wr_batched.hip", "wr_naive.hip"]
+HIP_SOURCES = ["wr_api.hip", "wr_kernels.hip", "wr_batched.hip", "wr_naive.hip", "wr_ffn.hip",
+               "wr_ffn_bf16.hip", "wr_ffn_f16.hip", "wr_ffn_f32.hip", "wr_ffn_i8.hip"]
 PROBE_SOURCE = "wr_probe.hip"
 PROBE_NAME = "libwr_probe.so"
 

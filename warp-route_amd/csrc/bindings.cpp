@@ -31,6 +31,7 @@
 #include <optional>
 
 #include "warp_route.h"
+#include "wr_ffn.h"
 
 namespace {
 
@@ -293,6 +294,256 @@ std::tuple<torch::Tensor, torch::Tensor> gate_topk(torch::Tensor hidden, torch::
   return {ids, ws};
 }
 
+// ---- dense gated FFN and int8 products (include/wr_ffn.h) -------------------
+int float_tag(const torch::Tensor& t, const char* name) {
+  if (t.scalar_type() == torch::kBFloat16) return WR_BF16;
+  if (t.scalar_type() == torch::kFloat32) return WR_F32;
+  if (t.scalar_type() == torch::kFloat16) return WR_F16;
+  TORCH_CHECK(false, name, " must be float32, float16 or bfloat16, got ", t.scalar_type());
+  return -1;
+}
+
+void check_operand(const torch::Tensor& t, const char* name, c10::ScalarType st,
+                   const torch::Device& dev, at::IntArrayRef shape) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA (HIP) tensor");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK(t.scalar_type() == st, name, " must be ", st, ", got ", t.scalar_type());
+  TORCH_CHECK(t.device() == dev, name, " must be on the device of the first argument");
+  TORCH_CHECK(t.sizes() == shape, name, " must have shape ", shape, ", got shape ", t.sizes());
+}
+
+void check_tokens(const torch::Tensor& x, const char* name) {
+  TORCH_CHECK(x.is_cuda(), name, " must be a CUDA (HIP) tensor");
+  TORCH_CHECK(x.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK(x.dim() == 2, name, " must have shape [rows, columns], got shape ", x.sizes());
+  TORCH_CHECK(x.size(0) <= INT32_MAX && x.size(1) >= 1, name, " has an unsupported shape ",
+              x.sizes());
+}
+
+void check_dims(int64_t h, int64_t I, int64_t most) {
+  TORCH_CHECK(h >= 1 && I >= 1 && h <= most && I <= most,
+              "dimensions must be in [1, ", most, "], got ", h, " and ", I);
+}
+
+// The C-ABI takes 16-byte aligned pointers: a view that starts elsewhere is copied.
+torch::Tensor aligned16(const torch::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone();
+}
+
+torch::Tensor scratch(size_t bytes, const torch::Device& dev) {
+  TORCH_CHECK(bytes > 0, "invalid shape for workspace sizing");
+  return torch::empty({(int64_t)bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
+}
+
+void* stream_of(const torch::Device& dev) {
+  return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+}
+
+wr_ffn_args ffn_args(const torch::Tensor& x, const torch::Tensor& wg, const torch::Tensor& wu,
+                     const torch::Tensor& wd) {
+  wr_ffn_args a{};
+  a.x = x.data_ptr();
+  a.w_gate = wg.data_ptr();
+  a.w_up = wu.data_ptr();
+  a.w_down = wd.data_ptr();
+  a.dtype = float_tag(x, "x");
+  a.batch_size = (int32_t)x.size(0);
+  a.hidden_dim = (int32_t)x.size(1);
+  a.intermediate_dim = (int32_t)wg.size(0);
+  return a;
+}
+
+void check_ffn(const torch::Tensor& x, const torch::Tensor& w_gate, const torch::Tensor& w_up,
+               const torch::Tensor& w_down) {
+  check_tokens(x, "x");
+  float_tag(x, "x");
+  TORCH_CHECK(w_gate.dim() == 2, "w_gate must have shape [intermediate_dim, hidden_dim], got shape ",
+              w_gate.sizes());
+  const int64_t h = x.size(1), I = w_gate.size(0);
+  check_dims(h, I, WR_FFN_MAX_DIM);
+  check_operand(w_gate, "w_gate", x.scalar_type(), x.device(), {I, h});
+  check_operand(w_up, "w_up", x.scalar_type(), x.device(), {I, h});
+  check_operand(w_down, "w_down", x.scalar_type(), x.device(), {h, I});
+}
+
+// gated_ffn_forward(x [T,h], w_gate [I,h], w_up [I,h], w_down [h,I], keep) -> [y], or
+// [y, g, u, a] with keep: what gated_ffn_backward reads.
+std::vector<torch::Tensor> gated_ffn_forward(torch::Tensor x, torch::Tensor w_gate,
+                                             torch::Tensor w_up, torch::Tensor w_down, bool keep) {
+  check_ffn(x, w_gate, w_up, w_down);
+  const torch::Device dev = x.device();
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  x = aligned16(x);
+  w_gate = aligned16(w_gate);
+  w_up = aligned16(w_up);
+  w_down = aligned16(w_down);
+  std::vector<torch::Tensor> out{torch::empty_like(x)};
+  wr_ffn_args a = ffn_args(x, w_gate, w_up, w_down);
+  if (keep) {
+    for (int i = 0; i < 3; ++i)
+      out.push_back(torch::empty({x.size(0), wr_ffn_saved_row(a.intermediate_dim)}, x.options()));
+    if (x.size(0) > 0) {
+      a.saved_gate = out[1].data_ptr();
+      a.saved_up = out[2].data_ptr();
+      a.saved_act = out[3].data_ptr();
+    }
+  }
+  if (x.size(0) == 0) return out;
+  a.out = out[0].data_ptr();
+  torch::Tensor ws = scratch(
+      wr_ffn_workspace_bytes(0, a.dtype, a.hidden_dim, a.intermediate_dim, a.batch_size), dev);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = (size_t)ws.numel();
+  check_status(wr_ffn_forward(&a, stream_of(dev)), "gated_ffn_forward");
+  return out;
+}
+
+// gated_ffn_backward(dy, x, w_gate, w_up, w_down, g, u, a, need [4]) -> [dx, dw_gate,
+// dw_up, dw_down], those not needed undefined.
+std::vector<std::optional<torch::Tensor>> gated_ffn_backward(
+    torch::Tensor dy, torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up,
+    torch::Tensor w_down, torch::Tensor g, torch::Tensor u, torch::Tensor act,
+    std::vector<bool> need) {
+  check_ffn(x, w_gate, w_up, w_down);
+  const torch::Device dev = x.device();
+  check_operand(dy, "dy", x.scalar_type(), dev, x.sizes());
+  const int64_t row = wr_ffn_saved_row((int)w_gate.size(0));
+  check_operand(g, "g", x.scalar_type(), dev, {x.size(0), row});
+  check_operand(u, "u", x.scalar_type(), dev, {x.size(0), row});
+  check_operand(act, "a", x.scalar_type(), dev, {x.size(0), row});
+  TORCH_CHECK(need.size() == 4, "need must hold 4 truth values, got ", need.size());
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  dy = aligned16(dy);
+  x = aligned16(x);
+  w_gate = aligned16(w_gate);
+  w_up = aligned16(w_up);
+  w_down = aligned16(w_down);
+  g = aligned16(g);
+  u = aligned16(u);
+  act = aligned16(act);
+  wr_ffn_args a = ffn_args(x, w_gate, w_up, w_down);
+  const torch::Tensor* like[4] = {&x, &w_gate, &w_up, &w_down};
+  void** slot[4] = {&a.dx, &a.dw_gate, &a.dw_up, &a.dw_down};
+  std::vector<std::optional<torch::Tensor>> out(4);
+  bool any = false;
+  for (int i = 0; i < 4; ++i) {
+    if (!need[i]) continue;
+    out[i] = torch::empty_like(*like[i]);
+    *slot[i] = out[i]->data_ptr();
+    any = true;
+  }
+  if (!any) return out;
+  a.dout = dy.data_ptr();
+  a.saved_gate = g.data_ptr();
+  a.saved_up = u.data_ptr();
+  a.saved_act = act.data_ptr();
+  torch::Tensor ws = scratch(
+      wr_ffn_workspace_bytes(1, a.dtype, a.hidden_dim, a.intermediate_dim, a.batch_size), dev);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = (size_t)ws.numel();
+  check_status(wr_ffn_backward(&a, stream_of(dev)), "gated_ffn_backward");
+  return out;
+}
+
+// quantize_int8(x [rows, cols]) -> (codes int8, scales fp32 [rows]).
+std::tuple<torch::Tensor, torch::Tensor> quantize_int8(torch::Tensor x) {
+  check_tokens(x, "x");
+  const int tag = float_tag(x, "x");
+  TORCH_CHECK(x.size(1) <= INT32_MAX, "x has an unsupported shape ", x.sizes());
+  const torch::Device dev = x.device();
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  x = aligned16(x);
+  torch::Tensor q = torch::empty_like(x, x.options().dtype(torch::kInt8));
+  torch::Tensor s = torch::empty({x.size(0)}, x.options().dtype(torch::kFloat32));
+  if (x.size(0) == 0) return {q, s};
+  check_status(wr_quantize_int8(x.data_ptr(), tag, (int)x.size(0), (int)x.size(1),
+                                q.data_ptr<int8_t>(), s.data_ptr<float>(), stream_of(dev)),
+               "quantize_int8");
+  return {q, s};
+}
+
+// int8_matmul(x int8 [M,K], x_scale [M], w int8 [N,K], w_scale [N], out_dtype) -> [M,N].
+torch::Tensor int8_matmul(torch::Tensor x, torch::Tensor x_scale, torch::Tensor w,
+                          torch::Tensor w_scale, py::object out_dtype) {
+  check_tokens(x, "x");
+  const torch::Device dev = x.device();
+  TORCH_CHECK(w.dim() == 2, "w must have shape [out_features, in_features], got shape ", w.sizes());
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  check_operand(x, "x", torch::kInt8, dev, {M, K});
+  check_operand(x_scale, "x_scale", torch::kFloat32, dev, {M});
+  check_operand(w, "w", torch::kInt8, dev, {N, K});
+  check_operand(w_scale, "w_scale", torch::kFloat32, dev, {N});
+  TORCH_CHECK(K <= WR_INT8_MAX_K && N >= 1 && N <= WR_FFN_MAX_DIM, "in_features must be in [1, ",
+              WR_INT8_MAX_K, "] and out_features in [1, ", WR_FFN_MAX_DIM, "], got ", K, " and ", N);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  x = aligned16(x);
+  w = aligned16(w);
+  torch::Tensor out = torch::empty(
+      {M, N}, torch::TensorOptions().dtype(torch::python::detail::py_object_to_dtype(out_dtype)).device(dev));
+  wr_int8_args a{};
+  a.out_dtype = float_tag(out, "out_dtype");
+  if (M == 0) return out;
+  a.x = x.data_ptr<int8_t>();
+  a.x_scale = x_scale.data_ptr<float>();
+  a.w = w.data_ptr<int8_t>();
+  a.w_scale = w_scale.data_ptr<float>();
+  a.out = out.data_ptr();
+  a.rows = (int32_t)M;
+  a.out_features = (int32_t)N;
+  a.in_features = (int32_t)K;
+  torch::Tensor ws = scratch(wr_int8_workspace_bytes(a.rows, a.out_features, a.in_features), dev);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = (size_t)ws.numel();
+  check_status(wr_int8_matmul(&a, stream_of(dev)), "int8_matmul");
+  return out;
+}
+
+// gated_ffn_int8(x [T,h], w_gate int8 [I,h], s_gate [I], w_up, s_up, w_down int8 [h,I],
+// s_down [h]) -> [T,h] in x's dtype.
+torch::Tensor gated_ffn_int8(torch::Tensor x, torch::Tensor w_gate, torch::Tensor s_gate,
+                             torch::Tensor w_up, torch::Tensor s_up, torch::Tensor w_down,
+                             torch::Tensor s_down) {
+  check_tokens(x, "x");
+  const int tag = float_tag(x, "x");
+  const torch::Device dev = x.device();
+  TORCH_CHECK(w_gate.dim() == 2, "w_gate must have shape [intermediate_dim, hidden_dim], got shape ",
+              w_gate.sizes());
+  const int64_t h = x.size(1), I = w_gate.size(0);
+  check_dims(h, I, WR_INT8_MAX_K);
+  check_operand(w_gate, "w_gate", torch::kInt8, dev, {I, h});
+  check_operand(s_gate, "s_gate", torch::kFloat32, dev, {I});
+  check_operand(w_up, "w_up", torch::kInt8, dev, {I, h});
+  check_operand(s_up, "s_up", torch::kFloat32, dev, {I});
+  check_operand(w_down, "w_down", torch::kInt8, dev, {h, I});
+  check_operand(s_down, "s_down", torch::kFloat32, dev, {h});
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  x = aligned16(x);
+  w_gate = aligned16(w_gate);
+  w_up = aligned16(w_up);
+  w_down = aligned16(w_down);
+  torch::Tensor out = torch::empty_like(x);
+  if (x.size(0) == 0) return out;
+  wr_ffn_int8_args a{};
+  a.x = x.data_ptr();
+  a.w_gate = w_gate.data_ptr<int8_t>();
+  a.s_gate = s_gate.data_ptr<float>();
+  a.w_up = w_up.data_ptr<int8_t>();
+  a.s_up = s_up.data_ptr<float>();
+  a.w_down = w_down.data_ptr<int8_t>();
+  a.s_down = s_down.data_ptr<float>();
+  a.out = out.data_ptr();
+  a.dtype = tag;
+  a.batch_size = (int32_t)x.size(0);
+  a.hidden_dim = (int32_t)h;
+  a.intermediate_dim = (int32_t)I;
+  torch::Tensor ws = scratch(
+      wr_ffn_int8_workspace_bytes(a.hidden_dim, a.intermediate_dim, a.batch_size), dev);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = (size_t)ws.numel();
+  check_status(wr_ffn_int8(&a, stream_of(dev)), "gated_ffn_int8");
+  return out;
+}
+
 void set_handoff_check(bool enabled) { g_check_handoff.store(enabled); }
 bool handoff_check() { return g_check_handoff.load(); }
 
@@ -331,6 +582,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gate_topk", &gate_topk, "Router logits, softmax and top-K", py::arg("hidden"),
         py::arg("gate_w"), py::arg("num_experts"), py::arg("hidden_dim"), py::arg("top_k"),
         py::arg("renormalize") = false);
+  m.def("gated_ffn_forward", &gated_ffn_forward,
+        "Dense gated FFN (fp32, fp16 or bf16); with keep also what its backward pass reads",
+        py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("w_down"),
+        py::arg("keep") = false);
+  m.def("gated_ffn_backward", &gated_ffn_backward, "Gradients of gated_ffn_forward", py::arg("dy"),
+        py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("w_down"), py::arg("g"),
+        py::arg("u"), py::arg("a"), py::arg("need"));
+  m.def("quantize_int8", &quantize_int8, "int8 codes and fp32 scales of rows", py::arg("x"));
+  m.def("int8_matmul", &int8_matmul, "Product of int8 codes, scaled per row and column",
+        py::arg("x"), py::arg("x_scale"), py::arg("w"), py::arg("w_scale"), py::arg("out_dtype"));
+  m.def("gated_ffn_int8", &gated_ffn_int8, "Dense gated FFN on int8 weights", py::arg("x"),
+        py::arg("w_gate"), py::arg("s_gate"), py::arg("w_up"), py::arg("s_up"), py::arg("w_down"),
+        py::arg("s_down"));
   m.def("set_handoff_check", &set_handoff_check,
         "Make fused_moe_forward synchronise and raise if its hand-off wait expired",
         py::arg("enabled"));

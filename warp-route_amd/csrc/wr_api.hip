@@ -259,6 +259,7 @@ WR_API const char* wr_status_str(int status) {
       return "a fused-kernel hand-off wait expired (the affected output rows are NaN)";
     case WR_EINVAL_SCRATCH:
       return "problem needs more workspace than the allocation-free entry point's 1 MiB scratch";
+    case WR_EINVAL_ALIGN: return "a pointer is not 16-byte aligned";
     case WR_EHIP: return "HIP runtime error";
     default: return "unknown status";
   }

@@ -1,0 +1,589 @@
+// Host side of the dense gated FFN and the int8 products (include/wr_ffn.h):
+// argument checks, workspace, the choice of tiles, and the row kernels around
+// the products (padded copies, quantisation).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "wr_device.h"
+#include "wr_ffn.h"
+#include "wr_ffn_internal.h"
+#include "wr_internal.h"
+
+namespace wr {
+namespace ffn {
+namespace {
+
+constexpr int64_t round_up(int64_t n, int64_t a) { return (n + a - 1) / a * a; }
+
+int elem_bytes(int dtype) { return dtype == WR_F32 ? 4 : 2; }
+bool float_dtype(int d) { return d == WR_F32 || d == WR_F16 || d == WR_BF16; }
+
+// ---- row kernels --------------------------------------------------------------
+// Rows of `bytes` bytes to rows of `ld` bytes, the tail zero: operands whose rows are
+// no whole 16-byte chunks, for the product kernels' 16-byte copies.  Bound by the
+// bytes; a thread assembles one 16-byte chunk from units of U, the element type.
+template <typename U>
+__global__ __launch_bounds__(256) void k_pad_rows(const U* __restrict__ src, char* __restrict__ dst,
+                                                  int64_t rows, int cols, int64_t ld) {
+  constexpr int N = 16 / sizeof(U);
+  typedef U V __attribute__((ext_vector_type(N)));
+  const int64_t per = ld / 16, total = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per;
+    const int c = (int)(i % per) * N;
+    const U* p = src + row * cols + c;
+    V v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = c + j < cols ? p[j] : (U)0;
+    *(V*)(dst + i * 16) = v;
+  }
+}
+
+__global__ __launch_bounds__(256) void k_fill_zero(uint32_t* __restrict__ p, int64_t words,
+                                                   char* __restrict__ tail, int tail_bytes) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words;
+       i += (int64_t)gridDim.x * 256)
+    p[i] = 0;
+  if (blockIdx.x == 0 && (int)threadIdx.x < tail_bytes) tail[threadIdx.x] = 0;
+}
+
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(f16 v) { return (float)v; }
+__device__ __forceinline__ float as_float(__bf16 v) { return (float)v; }
+
+// 127 x / m rounded to the nearest integer, ties to even, as the exact quotient
+// rounds.  In fp32 the quotient is off by less than 127 * 2^-22; where that could
+// reach a half-integer, or 127 x leaves the range, it is taken in 64 bits, whose
+// error (127 * 2^-53) is below the 2^-34 by which a quotient of two 24-bit
+// numbers misses a half-integer that it does not equal.
+__device__ __forceinline__ int code_of(float x, float m) {
+  const float t = x * 127.0f / m;
+  const float f = fabsf(t - rintf(t));
+  if (f > 0.4999f || !(m < 1e36f) || m < 1e-30f)
+    return (int)rint((double)x * 127.0 / (double)m);
+  return (int)rintf(t);
+}
+
+constexpr int kQuantThreads = 256;
+
+// One block per row: max |row|, then the codes (the row's second read comes from
+// cache).  HAVE_MAX: the maxima are there already (as fp32 bits).  codes rows are ldc
+// bytes apart, zero from cols on.  zero_max, when set, gets its word of the row cleared.
+template <typename T, bool HAVE_MAX>
+__global__ __launch_bounds__(kQuantThreads) void k_quantize(const T* __restrict__ x, int64_t ldx,
+                                                            int cols, const unsigned* row_max,
+                                                            int8_t* __restrict__ codes, int64_t ldc,
+                                                            float* __restrict__ scales,
+                                                            unsigned* __restrict__ zero_max,
+                                                            bool vec) {
+  __shared__ unsigned part[kQuantThreads / 64];
+  const int64_t row = blockIdx.x;
+  const T* p = x + row * ldx;
+  constexpr int N = 16 / sizeof(T);
+  typedef T V __attribute__((ext_vector_type(N)));
+  unsigned mx = 0;
+  if (HAVE_MAX) {
+    mx = row_max[row];
+  } else {
+    if (vec) {
+      for (int c = threadIdx.x * N; c < cols; c += kQuantThreads * N) {
+        const V v = *(const V*)(p + c);
+#pragma unroll
+        for (int i = 0; i < N; ++i) mx = max(mx, __float_as_uint(as_float(v[i])) & 0x7fffffffu);
+      }
+    } else {
+      for (int c = threadIdx.x; c < cols; c += kQuantThreads)
+        mx = max(mx, __float_as_uint(as_float(p[c])) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) mx = max(mx, (unsigned)__shfl_xor((int)mx, d));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kQuantThreads / 64; ++i) mx = max(mx, part[i]);
+  }
+  const bool finite = mx < 0x7f800000u;
+  const float m = __uint_as_float(mx);
+  if (threadIdx.x == 0) {
+    scales[row] = !finite ? __builtin_nanf("") : mx == 0 ? 1.0f : m / 127.0f;
+    if (zero_max != nullptr) zero_max[row] = 0;
+  }
+  const bool live = finite && mx != 0;
+  int8_t* q = codes + row * ldc;
+  typedef int8_t Q __attribute__((ext_vector_type(N)));
+  if (vec && ldc % N == 0) {
+    for (int c = threadIdx.x * N; c < (int)ldc; c += kQuantThreads * N) {
+      Q o;
+      if (c < cols) {
+        const V v = *(const V*)(p + c);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          o[i] = live && c + i < cols ? (int8_t)code_of(as_float(v[i]), m) : (int8_t)0;
+      } else {
+        o = Q{};
+      }
+      *(Q*)(q + c) = o;
+    }
+  } else {
+    for (int c = threadIdx.x; c < (int)ldc; c += kQuantThreads)
+      q[c] = live && c < cols ? (int8_t)code_of(as_float(p[c]), m) : (int8_t)0;
+  }
+}
+
+template <bool HAVE_MAX>
+hipError_t launch_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols,
+                           const unsigned* row_max, int8_t* codes, int64_t ldc, float* scales,
+                           unsigned* zero_max, hipStream_t s) {
+  if (rows == 0) return hipSuccess;
+  const int n = 16 / elem_bytes(dtype);
+  // Vector reads may pass cols inside a row's padding, never the row.
+  const bool vec = ldx % n == 0 && round_up(cols, n) <= ldx &&
+                   reinterpret_cast<uintptr_t>(codes) % 16 == 0;
+  if (dtype == WR_F32)
+    k_quantize<float, HAVE_MAX><<<rows, kQuantThreads, 0, s>>>(
+        (const float*)x, ldx, cols, row_max, codes, ldc, scales, zero_max, vec);
+  else if (dtype == WR_F16)
+    k_quantize<f16, HAVE_MAX><<<rows, kQuantThreads, 0, s>>>((const f16*)x, ldx, cols, row_max,
+                                                             codes, ldc, scales, zero_max, vec);
+  else
+    k_quantize<__bf16, HAVE_MAX><<<rows, kQuantThreads, 0, s>>>(
+        (const __bf16*)x, ldx, cols, row_max, codes, ldc, scales, zero_max, vec);
+  return hipGetLastError();
+}
+
+unsigned row_blocks(int64_t threads) {
+  return (unsigned)std::min<int64_t>((threads + 255) / 256, 8192);
+}
+
+hipError_t launch_pad(const void* src, char* dst, int64_t rows, int cols, int64_t ld, int es,
+                      hipStream_t s) {
+  const unsigned blocks = row_blocks(rows * (ld / 16));
+  if (blocks == 0) return hipSuccess;
+  if (es == 4)
+    k_pad_rows<uint32_t><<<blocks, 256, 0, s>>>((const uint32_t*)src, dst, rows, cols, ld);
+  else if (es == 2)
+    k_pad_rows<uint16_t><<<blocks, 256, 0, s>>>((const uint16_t*)src, dst, rows, cols, ld);
+  else
+    k_pad_rows<uint8_t><<<blocks, 256, 0, s>>>((const uint8_t*)src, dst, rows, cols, ld);
+  return hipGetLastError();
+}
+
+hipError_t launch_zero(void* p, int64_t bytes, hipStream_t s) {
+  if (bytes == 0) return hipSuccess;
+  const int64_t words = bytes / 4;
+  k_fill_zero<<<std::max(1u, row_blocks(words)), 256, 0, s>>>(
+      (uint32_t*)p, words, (char*)p + words * 4, (int)(bytes - words * 4));
+  return hipGetLastError();
+}
+
+// ---- the choice of tiles --------------------------------------------------------
+// A product's time is taken as rounds x (steps of a slice x time of a step + the
+// tile's fixed part) + what splitting costs; the shape and number of slices with the
+// least is chosen.
+struct ShapeCost {
+  int bm, bn, per_cu;  // tile, blocks a CU holds
+  float step;          // us a K step of a tile takes with per_cu blocks on the CU
+  float fixed;         // us per tile: first copies, epilogue
+};
+constexpr ShapeCost kCost[kShapes] = {
+    {256, 256, 1, 1.5f, 4.0f}, {128, 128, 2, 0.9f, 3.0f}, {64, 256, 2, 1.1f, 3.0f}};
+constexpr int kCUs = 256;
+constexpr int kMaxSlices = 32;
+constexpr int64_t kMaxPartBytes = (int64_t)256 << 20;
+
+struct Plan {
+  int shape, slices, tiles_m, tiles_n;
+  int64_t ldp;
+  size_t part_bytes;
+};
+
+// M x N x K per problem; gated: N columns of each of two matrices.
+Plan plan_of(int M, int N, int K, int es, int nseg, int nprob, bool gated) {
+  const int kb = 128 / es;
+  const int steps = (K + kb - 1) / kb * nseg;
+  const float rate = es == 4 ? 8.0f : 1.0f;  // fp32 steps: 16 times the time of half the K
+  Plan best{};
+  float best_us = 0;
+  const int64_t ldp = round_up(N, 64);
+  for (int shape = 0; shape < kShapes; ++shape) {
+    const ShapeCost& c = kCost[shape];
+    const int64_t tm = (M + c.bm - 1) / c.bm, bn = gated ? c.bn / 2 : c.bn;
+    const int64_t tn = (N + bn - 1) / bn;
+    for (int S = 1; S <= kMaxSlices; S *= 2) {
+      const size_t part = S == 1 ? 0 : (size_t)S * nprob * M * ldp * 4 * (gated ? 2 : 1);
+      if (S > 1 && (steps / S < 4 || part > (size_t)kMaxPartBytes)) break;
+      const int64_t blocks = tm * tn * nprob * S;
+      const int64_t rounds = (blocks + (int64_t)kCUs * c.per_cu - 1) / ((int64_t)kCUs * c.per_cu);
+      const int per = (steps + S - 1) / S;
+      const float us = rounds * (per * c.step * rate + c.fixed) +
+                       (S == 1 ? 0.0f : 4.0f + (float)part * 2 / 4e6f);
+      if (best.tiles_m == 0 || us < best_us) {
+        best = {shape, S, (int)tm, (int)tn, ldp, part};
+        best_us = us;
+      }
+    }
+  }
+  return best;
+}
+
+// ---- a call: workspace and launches from the same code --------------------------
+// With `ws` null nothing is launched and `used` counts the workspace.
+struct Call {
+  char* ws;
+  hipStream_t stream;
+  int dtype;  // of the products' operands, unless int8
+  bool int8;
+  size_t used = 0, part_at = 0, part_bytes = 0;
+  hipError_t err = hipSuccess;
+
+  bool dry() const { return ws == nullptr; }
+  int es() const { return int8 ? 1 : elem_bytes(dtype); }
+  char* take(int64_t bytes) {
+    char* p = dry() ? nullptr : ws + used;
+    used += align_up((size_t)bytes, kWsAlign);
+    return p;
+  }
+  void check(hipError_t e) {
+    if (err == hipSuccess) err = e;
+  }
+  bool go() const { return !dry() && err == hipSuccess; }
+
+  // An operand matrix with whole 16-byte rows: itself, or a padded copy.
+  struct Mat {
+    const char* p;
+    int64_t ld;  // bytes
+  };
+  Mat rows16(const void* p, int64_t rows, int cols) {
+    const int64_t bytes = (int64_t)cols * es(), ld = round_up(bytes, 16);
+    if (ld == bytes) return {(const char*)p, ld};
+    char* c = take(rows * ld);
+    if (go()) check(launch_pad(p, c, rows, cols, ld, es(), stream));
+    return {c, ld};
+  }
+
+  // The slices' sums share one region (products of a call run one after another).
+  void reserve_part(const Plan& pl) { part_bytes = std::max(part_bytes, pl.part_bytes); }
+
+  void product(GemmArgs g, int form) {
+    const bool gated = form == kFormGated || form == kFormGatedMax;
+    if (g.M == 0 || g.N == 0) return;
+    const Plan pl = plan_of(g.M, g.N, g.K, es(), g.nseg, g.nprob, gated);
+    reserve_part(pl);
+    if (!go()) return;
+    g.slices = pl.slices;
+    g.tiles_m = pl.tiles_m;
+    g.tiles_n = pl.tiles_n;
+    g.ldp = pl.ldp;
+    g.part = ws + part_at;
+    const int oes = int8 ? elem_bytes(g.out_dtype) : es();
+    g.vec = g.ldo * oes % 16 == 0;
+    check(int8 ? launch_i8(g, pl.shape, form, stream)
+          : dtype == WR_F32 ? launch_f32(g, pl.shape, form, stream)
+          : dtype == WR_F16 ? launch_f16(g, pl.shape, form, stream)
+                            : launch_bf16(g, pl.shape, form, stream));
+  }
+};
+
+GemmArgs gemm(const Call::Mat& a, const Call::Mat& b, int M, int N, int K) {
+  GemmArgs g{};
+  g.a[0] = g.a[1] = a.p;
+  g.b[0] = g.b[1] = b.p;
+  g.lda = a.ld;
+  g.ldb = b.ld;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.nseg = g.nprob = g.slices = 1;
+  return g;
+}
+
+void run_forward(Call& c, const wr_ffn_args& a) {
+  const int T = a.batch_size, h = a.hidden_dim, I = a.intermediate_dim;
+  const int64_t Ip = round_up(I, 64);
+  const bool keep = a.saved_act != nullptr;
+  const Call::Mat x = c.rows16(a.x, T, h);
+  const Call::Mat wg = c.rows16(a.w_gate, I, h), wu = c.rows16(a.w_up, I, h);
+  const Call::Mat wd = c.rows16(a.w_down, h, I);
+  char* own = c.take((int64_t)T * Ip * c.es());  // sized whether saved or not
+  const Call::Mat act{keep ? (const char*)a.saved_act : own, Ip * c.es()};
+
+  GemmArgs g = gemm(x, wg, T, I, h);
+  g.b[1] = wu.p;
+  g.ldi = Ip;
+  g.out[0] = const_cast<char*>(act.p);
+  g.out[1] = a.saved_gate;
+  g.out[2] = a.saved_up;
+  c.product(g, kFormGated);
+
+  g = gemm(act, wd, T, h, I);
+  g.out[0] = a.out;
+  g.ldo = h;
+  c.product(g, kFormKcKc);
+}
+
+void run_backward(Call& c, const wr_ffn_args& a, bool dx, bool dwg, bool dwu, bool dwd) {
+  const int T = a.batch_size, h = a.hidden_dim, I = a.intermediate_dim;
+  const int64_t Ip = round_up(I, 64), ldi = Ip * c.es();
+  const bool din = dx || dwg || dwu;
+  const Call::Mat dy = c.rows16(a.dout, T, h);
+  GemmArgs g;
+  if (din) {
+    char* dgate = c.take(T * ldi);
+    char* dup = c.take(T * ldi);
+    const Call::Mat wd = c.rows16(a.w_down, h, I);
+    g = gemm(dy, wd, T, I, h);
+    g.ldi = Ip;
+    g.in[0] = a.saved_gate;
+    g.in[1] = a.saved_up;
+    g.out[0] = dgate;
+    g.out[1] = dup;
+    c.product(g, kFormGateGrad);
+    if (dx) {
+      const Call::Mat wg = c.rows16(a.w_gate, I, h), wu = c.rows16(a.w_up, I, h);
+      g = gemm({dgate, ldi}, wg, T, h, I);
+      g.a[1] = dup;
+      g.b[1] = wu.p;
+      g.nseg = 2;
+      g.out[0] = a.dx;
+      g.ldo = h;
+      c.product(g, kFormKcKs);
+    }
+    if (dwg || dwu) {
+      const Call::Mat x = c.rows16(a.x, T, h);
+      g = gemm({dwg ? dgate : dup, ldi}, x, I, h, T);
+      g.a[1] = dup;
+      g.nprob = dwg && dwu ? 2 : 1;
+      g.out[0] = dwg ? a.dw_gate : a.dw_up;
+      g.out[1] = a.dw_up;
+      g.ldo = h;
+      c.product(g, kFormKsKs);
+    }
+  }
+  if (dwd) {
+    g = gemm(dy, {(const char*)a.saved_act, ldi}, h, I, T);
+    g.out[0] = a.dw_down;
+    g.ldo = I;
+    c.product(g, kFormKsKs);
+  }
+}
+
+void run_int8(Call& c, const wr_int8_args& a) {
+  const Call::Mat x = c.rows16(a.x, a.rows, a.in_features);
+  const Call::Mat w = c.rows16(a.w, a.out_features, a.in_features);
+  GemmArgs g = gemm(x, w, a.rows, a.out_features, a.in_features);
+  g.out[0] = a.out;
+  g.ldo = a.out_features;
+  g.out_dtype = a.out_dtype;
+  g.row_scale = a.x_scale;
+  g.col_scale[0] = a.w_scale;
+  c.product(g, kFormScale);
+}
+
+void run_ffn_int8(Call& c, const wr_ffn_int8_args& a) {
+  const int T = a.batch_size, h = a.hidden_dim, I = a.intermediate_dim;
+  const int64_t Ip = round_up(I, 64), hp = round_up(h, 16);
+  int8_t* xq = (int8_t*)c.take(T * hp);
+  float* sx = (float*)c.take((int64_t)T * 4);
+  unsigned* amax = (unsigned*)c.take((int64_t)T * 4);
+  float* act = (float*)c.take(T * Ip * 4);
+  int8_t* aq = (int8_t*)c.take(T * Ip);
+  float* sa = (float*)c.take((int64_t)T * 4);
+  const Call::Mat wg = c.rows16(a.w_gate, I, h), wu = c.rows16(a.w_up, I, h);
+  const Call::Mat wd = c.rows16(a.w_down, h, I);
+  if (c.go())
+    c.check(launch_quantize<false>(a.x, a.dtype, h, T, h, nullptr, xq, hp, sx, amax, c.stream));
+  GemmArgs g = gemm({(const char*)xq, hp}, wg, T, I, h);
+  g.b[1] = wu.p;
+  g.ldi = Ip;
+  g.out[0] = act;
+  g.row_scale = sx;
+  g.col_scale[0] = a.s_gate;
+  g.col_scale[1] = a.s_up;
+  g.row_max = amax;
+  c.product(g, kFormGatedMax);
+  if (c.go())
+    c.check(launch_quantize<true>(act, WR_F32, Ip, T, I, amax, aq, Ip, sa, nullptr, c.stream));
+  g = gemm({(const char*)aq, Ip}, wd, T, h, I);
+  g.out[0] = a.out;
+  g.ldo = h;
+  g.out_dtype = a.dtype;
+  g.row_scale = sa;
+  g.col_scale[0] = a.s_down;
+  c.product(g, kFormScale);
+}
+
+// Runs `body` once dry for the workspace's size, then for real.  The slices' sums lie
+// behind everything else.
+template <typename Body>
+size_t workspace_of(int dtype, bool int8, Body body) {
+  Call c{nullptr, nullptr, dtype, int8};
+  body(c);
+  return std::max<size_t>(kWsAlign, c.used + c.part_bytes);
+}
+
+template <typename Body>
+int run(int dtype, bool int8, void* ws, size_t ws_bytes, void* stream, Body body) {
+  Call c{nullptr, nullptr, dtype, int8};
+  body(c);
+  if (ws == nullptr || ws_bytes < std::max<size_t>(kWsAlign, c.used + c.part_bytes))
+    return WR_EINVAL_WORKSPACE;
+  Call r{(char*)ws, (hipStream_t)stream, dtype, int8};
+  r.part_at = c.used;
+  body(r);
+  return r.err == hipSuccess ? WR_OK : WR_EHIP;
+}
+
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int check_ffn(const wr_ffn_args* a) {
+  if (a == nullptr) return WR_EINVAL_NULL;
+  if (!float_dtype(a->dtype)) return WR_EINVAL_DTYPE;
+  if (a->hidden_dim < 1 || a->intermediate_dim < 1 || a->hidden_dim > WR_FFN_MAX_DIM ||
+      a->intermediate_dim > WR_FFN_MAX_DIM)
+    return WR_EINVAL_SHAPE;
+  if (a->batch_size < 0) return WR_EINVAL_BATCH;
+  for (const void* p : {a->x, a->w_gate, a->w_up, a->w_down, (const void*)a->workspace,
+                        (const void*)a->saved_gate, (const void*)a->saved_up,
+                        (const void*)a->saved_act})
+    if (!aligned(p)) return WR_EINVAL_ALIGN;
+  return WR_OK;
+}
+
+}  // namespace
+}  // namespace ffn
+}  // namespace wr
+
+using namespace wr::ffn;
+
+extern "C" {
+
+int64_t wr_ffn_saved_row(int I) { return I < 1 || I > WR_FFN_MAX_DIM ? 0 : round_up(I, 64); }
+
+size_t wr_ffn_workspace_bytes(int backward, int dtype, int h, int I, int T) {
+  wr_ffn_args a{};
+  a.dtype = dtype;
+  a.hidden_dim = h;
+  a.intermediate_dim = I;
+  a.batch_size = T;
+  if (check_ffn(&a) != WR_OK) return 0;
+  return workspace_of(dtype, false, [&](Call& c) {
+    if (backward)
+      run_backward(c, a, true, true, true, true);
+    else
+      run_forward(c, a);
+  });
+}
+
+int wr_ffn_forward(const wr_ffn_args* a, void* stream) {
+  if (const int st = check_ffn(a)) return st;
+  if (a->batch_size == 0) return WR_OK;
+  if (!a->x || !a->w_gate || !a->w_up || !a->w_down || !a->out) return WR_EINVAL_NULL;
+  const int kept = (a->saved_gate != nullptr) + (a->saved_up != nullptr) + (a->saved_act != nullptr);
+  if (kept != 0 && kept != 3) return WR_EINVAL_NULL;
+  if (!aligned(a->out)) return WR_EINVAL_ALIGN;
+  return run(a->dtype, false, a->workspace, a->workspace_bytes, stream,
+             [&](Call& c) { run_forward(c, *a); });
+}
+
+int wr_ffn_backward(const wr_ffn_args* a, void* stream) {
+  if (const int st = check_ffn(a)) return st;
+  for (const void* p : {a->dout, (const void*)a->dx, (const void*)a->dw_gate,
+                        (const void*)a->dw_up, (const void*)a->dw_down})
+    if (!aligned(p)) return WR_EINVAL_ALIGN;
+  const bool dx = a->dx != nullptr, dwg = a->dw_gate != nullptr, dwu = a->dw_up != nullptr,
+             dwd = a->dw_down != nullptr;
+  if (a->batch_size == 0) {  // no tokens: the weights' gradients are zero
+    const int64_t n = (int64_t)a->hidden_dim * a->intermediate_dim *
+                      wr::ffn::elem_bytes(a->dtype);
+    for (void* p : {a->dw_gate, a->dw_up, a->dw_down})
+      if (p != nullptr && launch_zero(p, n, (hipStream_t)stream) != hipSuccess) return WR_EHIP;
+    return WR_OK;
+  }
+  if (!a->dout || ((dwg || dwu) && !a->x) || (dx && (!a->w_gate || !a->w_up)) ||
+      ((dx || dwg || dwu) && (!a->w_down || !a->saved_gate || !a->saved_up)) ||
+      (dwd && !a->saved_act))
+    return WR_EINVAL_NULL;
+  return run(a->dtype, false, a->workspace, a->workspace_bytes, stream,
+             [&](Call& c) { run_backward(c, *a, dx, dwg, dwu, dwd); });
+}
+
+int wr_quantize_int8(const void* x, int dtype, int rows, int cols, int8_t* codes, float* scales,
+                     void* stream) {
+  if (!float_dtype(dtype)) return WR_EINVAL_DTYPE;
+  if (rows < 0) return WR_EINVAL_BATCH;
+  if (cols < 1) return WR_EINVAL_SHAPE;
+  if (rows == 0) return WR_OK;
+  if (!x || !codes || !scales) return WR_EINVAL_NULL;
+  if (!aligned(x) || !aligned(codes) || !aligned(scales)) return WR_EINVAL_ALIGN;
+  return launch_quantize<false>(x, dtype, cols, rows, cols, nullptr, codes, cols, scales, nullptr,
+                                (hipStream_t)stream) == hipSuccess
+             ? WR_OK
+             : WR_EHIP;
+}
+
+static int check_int8(const wr_int8_args* a) {
+  if (a == nullptr) return WR_EINVAL_NULL;
+  if (!float_dtype(a->out_dtype)) return WR_EINVAL_DTYPE;
+  if (a->out_features < 1 || a->in_features < 1 || a->out_features > WR_FFN_MAX_DIM ||
+      a->in_features > WR_INT8_MAX_K)
+    return WR_EINVAL_SHAPE;
+  if (a->rows < 0) return WR_EINVAL_BATCH;
+  return WR_OK;
+}
+
+size_t wr_int8_workspace_bytes(int rows, int out_features, int in_features) {
+  wr_int8_args a{};
+  a.rows = rows;
+  a.out_features = out_features;
+  a.in_features = in_features;
+  if (check_int8(&a) != WR_OK) return 0;
+  return workspace_of(WR_F32, true, [&](Call& c) { run_int8(c, a); });
+}
+
+int wr_int8_matmul(const wr_int8_args* a, void* stream) {
+  if (const int st = check_int8(a)) return st;
+  if (a->rows == 0) return WR_OK;
+  if (!a->x || !a->x_scale || !a->w || !a->w_scale || !a->out) return WR_EINVAL_NULL;
+  for (const void* p : {(const void*)a->x, (const void*)a->w, (const void*)a->out,
+                        (const void*)a->workspace})
+    if (!aligned(p)) return WR_EINVAL_ALIGN;
+  return run(WR_F32, true, a->workspace, a->workspace_bytes, stream,
+             [&](Call& c) { run_int8(c, *a); });
+}
+
+static int check_ffn_int8(const wr_ffn_int8_args* a) {
+  if (a == nullptr) return WR_EINVAL_NULL;
+  if (!float_dtype(a->dtype)) return WR_EINVAL_DTYPE;
+  if (a->hidden_dim < 1 || a->intermediate_dim < 1 || a->hidden_dim > WR_INT8_MAX_K ||
+      a->intermediate_dim > WR_INT8_MAX_K)
+    return WR_EINVAL_SHAPE;
+  if (a->batch_size < 0) return WR_EINVAL_BATCH;
+  return WR_OK;
+}
+
+size_t wr_ffn_int8_workspace_bytes(int h, int I, int T) {
+  wr_ffn_int8_args a{};
+  a.hidden_dim = h;
+  a.intermediate_dim = I;
+  a.batch_size = T;
+  if (check_ffn_int8(&a) != WR_OK) return 0;
+  return workspace_of(WR_F32, true, [&](Call& c) { run_ffn_int8(c, a); });
+}
+
+int wr_ffn_int8(const wr_ffn_int8_args* a, void* stream) {
+  if (const int st = check_ffn_int8(a)) return st;
+  if (a->batch_size == 0) return WR_OK;
+  if (!a->x || !a->w_gate || !a->s_gate || !a->w_up || !a->s_up || !a->w_down || !a->s_down ||
+      !a->out)
+    return WR_EINVAL_NULL;
+  for (const void* p : {(const void*)a->x, (const void*)a->w_gate, (const void*)a->w_up,
+                        (const void*)a->w_down, (const void*)a->out, (const void*)a->workspace})
+    if (!aligned(p)) return WR_EINVAL_ALIGN;
+  return run(a->dtype, true, a->workspace, a->workspace_bytes, stream,
+             [&](Call& c) { run_ffn_int8(c, *a); });
+}
+
+}  // extern "C"

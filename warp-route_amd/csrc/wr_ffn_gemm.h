@@ -1,0 +1,586 @@
+// Matrix products of the dense gated FFN, C[m][n] = sum_k A(m, k) B(n, k), on
+// the gfx950 matrix cores, with the FFN's elementwise parts in the epilogue.
+//
+// One kernel template covers every product of the forward and backward pass.
+// An operand is either K-contiguous (rows of m or n, "KC") or K-strided (rows
+// of k, "KS"), so that no operand is transposed in memory:
+//
+//   gate, up    A = x      KC  B = Wg, Wu    KC  -> a = silu(g) u (and g, u)
+//   down        A = a      KC  B = Wd        KC  -> y
+//   d(act)      A = dy     KC  B = Wd        KS  -> dg, du from g, u
+//   dx          A = dg, du KC  B = Wg, Wu    KS  -> dx (K runs over both)
+//   dWg, dWu    A = dg, du KS  B = x         KS  (two problems of one launch)
+//   dWd         A = dy     KS  B = a         KS
+//   int8        A = codes  KC  B = codes     KC  -> y, or a with its row maxima
+//
+// Tiles.  A K step is 128 bytes of K: 64 16-bit elements, 128 int8, 32 fp32.
+// Both operand tiles of a step are copied from memory straight into LDS
+// (buffer_load ... lds, 16 bytes a lane), into one of two buffers while the
+// other is multiplied.  The copy's buffer descriptor ends at the operand's
+// last element, so rows past the end arrive as zeros without a branch; K
+// tails and column tails give their lanes an offset behind the descriptor.
+//
+// A wave owns MT x 4 tiles of 16 x 16.  B is the MFMA's first operand, so a
+// lane's four accumulators are four consecutive n of one m.  For KC B the
+// LDS rows of a wave's 64 n are dealt to the MFMA rows so that a lane's 4
+// tiles together hold 16 consecutive n (gated: 8 of gate and the same 8 of
+// up): stores are whole 16-byte vectors.
+//
+// LDS positions are swizzled in 16-byte chunks (KC), 32-byte (KS, 16-bit) or
+// 64-byte ones (KS, fp32), chosen so that the lanes one LDS pass serves hit
+// different banks; the copy applies the swizzle by choosing its source
+// address, since its LDS side is linear.  16-bit KS tiles are read with the
+// transposing LDS read (4 rows of k x 16 columns per 16 lanes).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "wr_device.h"
+#include "wr_ffn_internal.h"
+
+namespace wr {
+namespace ffn {
+
+typedef __bf16 bf16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kStepBytes = 128;  // bytes of K per step
+constexpr unsigned kOutside = 0x80000000u;  // offset behind every descriptor
+
+// ---- one 16 x 16 tile product over 64 bytes of K ---------------------------
+template <typename T>
+struct Mma;
+template <>
+struct Mma<bf16> {
+  typedef f32x4 Acc;
+  static __device__ __forceinline__ Acc go(u32x4 a, u32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<f16> {
+  typedef f32x4 Acc;
+  static __device__ __forceinline__ Acc go(u32x4 a, u32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<int8_t> {
+  typedef i32x4 Acc;
+  static __device__ __forceinline__ Acc go(u32x4 a, u32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a),
+                                                 __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+  }
+};
+// fp32: lane group q holds k = 4 q .. 4 q + 3, one element per MFMA.
+template <>
+struct Mma<float> {
+  typedef f32x4 Acc;
+  static __device__ __forceinline__ Acc go(u32x4 a, u32x4 b, Acc c) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// ---- copying one operand's K step into LDS ---------------------------------
+// Swizzle keys: KC tiles are [row][128 bytes], KS tiles [k][ROWS elements].
+template <bool NSIDE>
+__device__ __forceinline__ int kc_key(int row) {  // xor of the 16-byte chunk index
+  // M side: 16 lanes read 16 consecutive rows.  N side: rows 16 q + 4 t + i, q, i < 4.
+  return NSIDE ? (((row >> 1) & 1) | (((row >> 4) & 3) << 1)) : ((row >> 1) & 7);
+}
+template <int ES, int ROWS>
+__device__ __forceinline__ int ks_key(int k) {  // xor of the 32- (64-) byte chunk index
+  if (ES == 4) return (k >> 2) & 3;
+  return ROWS >= 128 ? ((k & 3) | (((k >> 3) & 1) << 2)) : (((k >> 1) & 1) | (((k >> 3) & 1) << 1));
+}
+
+// Lane-to-source mapping of a tile of ROWS m or n (times one K step), copied by
+// NW waves, PER copies of 1 KB each per wave.
+template <typename T, int ROWS, int NW, bool KS, bool NSIDE, bool GATED>
+struct TileCopy {
+  static constexpr int ES = sizeof(T);
+  static constexpr int kBytes = ROWS * kStepBytes;
+  static constexpr int kCopies = kBytes / 1024;
+  static constexpr int PER = (kCopies + NW - 1) / NW;
+  static constexpr int kStep = kStepBytes / ES;     // K elements per step
+  static constexpr int EPC = 16 / ES;               // elements per chunk
+  unsigned voff[PER];
+
+  // Chunk of this lane in copy j, as a k offset (KC).
+  static __device__ __forceinline__ int k_chunk(int j, int wave, int lane) {
+    const int row = (j * NW + wave) * 8 + (lane >> 3);
+    return (lane & 7) ^ kc_key<NSIDE>(row);
+  }
+
+  // cols: KS only, m (n) elements left from the tile's first one.
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int cols) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (KS) {
+        constexpr int CPR = ROWS * ES / 16;  // chunks per k row
+        const int L = (j * NW + wave) * 64 + lane;
+        const int k = L / CPR, p = L % CPR;
+        constexpr int G = ES == 4 ? 4 : 2;  // chunks per swizzle unit
+        const int c = ((p / G) ^ ks_key<ES, ROWS>(k)) * G + p % G;
+        voff[j] = c * EPC < cols ? (unsigned)(k * ld + c * 16) : kOutside;
+      } else {
+        int row = (j * NW + wave) * 8 + (lane >> 3);
+        if (GATED) row = (row >> 4) * 8 + (row & 7);  // rows 8..15 of 16 are the other matrix's
+        voff[j] = (unsigned)(row * ld + k_chunk(j, wave, lane) * 16);
+      }
+    }
+  }
+
+  // base: the tile's first byte at this K step; end: the operand's bytes from
+  // there on; krem: K elements left at this step.
+  __device__ __forceinline__ void issue(char* lds, const char* base, int64_t end, int krem,
+                                        int wave, int lane) const {
+    const int records = end > 0x7fffffff ? 0x7fffffff : (int)end;
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, records, 0x00020000);
+    const bool tail = !KS && krem < kStep;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (kCopies % NW != 0 && j * NW + wave >= kCopies) break;
+      unsigned v = voff[j];
+      if (tail && k_chunk(j, wave, lane) * EPC >= krem) v = kOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          r, (__attribute__((address_space(3))) void*)(lds + (j * NW + wave) * 1024), 16, (int)v, 0,
+          0, 0);
+    }
+  }
+};
+
+// ---- reading a wave's fragments from LDS -----------------------------------
+__device__ __forceinline__ u32x4 lds_b128(const char* p) {
+  return *(const __attribute__((address_space(3))) u32x4*)p;
+}
+
+// S subtiles of 16 m (n) from subtile sub0 of a tile of ROWS.
+template <typename T, int ROWS, int S, bool KS, bool NSIDE>
+struct Frag {
+  static constexpr int ES = sizeof(T);
+  static constexpr int RB = ROWS * ES;  // bytes per k row (KS)
+  int addr[KS ? S : 2];
+
+  __device__ __forceinline__ void init(int sub0, int lane) {
+    const int r = lane & 15, q = lane >> 4;
+    if constexpr (!KS) {
+      // M side: row 16 s + r.  N side: subtile t's row r = 4 q' + i is LDS row 16 q' + 4 t + i.
+      const int row = sub0 * 16 + (NSIDE ? (r >> 2) * 16 + (r & 3) : r);
+      const int key = kc_key<NSIDE>(row);
+      addr[0] = row * kStepBytes + (q ^ key) * 16;
+      addr[1] = row * kStepBytes + ((4 + q) ^ key) * 16;
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (ES == 2) {
+          const int k = 8 * q + (r >> 2);
+          addr[s] = k * RB + ((sub0 + s) ^ ks_key<ES, ROWS>(k)) * 32 + (r & 3) * 8;
+        } else {
+          const int k = 4 * q;
+          addr[s] = k * RB + ((sub0 + s) ^ ks_key<ES, ROWS>(k)) * 64 + r * 4;
+        }
+      }
+    }
+  }
+
+  // Fragment of subtile s, 64-byte half kk of the K step.
+  __device__ __forceinline__ u32x4 get(char* tile, int s, int kk) const {
+    if constexpr (!KS) {
+      return lds_b128(tile + addr[kk] + s * (NSIDE ? 4 : 16) * kStepBytes);
+    } else if constexpr (ES == 2) {
+      typedef __attribute__((address_space(3))) s16x4* P;
+      char* a = tile + addr[s] + kk * 32 * RB;
+      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)a));
+      const u32x2 hi =
+          __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(a + 4 * RB)));
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+      const char* a = tile + addr[s] + kk * 16 * RB;
+      u32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = *(const __attribute__((address_space(3))) uint32_t*)(a + j * RB);
+      return v;
+    }
+  }
+};
+
+// ---- epilogues --------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ T to_out(float v) {
+  return (T)v;
+}
+
+__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+// g * sigmoid(g)
+__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
+
+// N consecutive elements at p[0..N), of which the first `left` exist.  VEC: p is
+// aligned to its N elements.
+template <typename T, int N>
+__device__ __forceinline__ void store_run(T* p, const float* v, int left, bool vec) {
+  if (vec && left >= N) {
+    typedef T V __attribute__((ext_vector_type(N)));
+    V o;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = to_out<T>(v[i]);
+    *(V*)p = o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < left) p[i] = to_out<T>(v[i]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const T* p) {
+  typedef T V __attribute__((ext_vector_type(4)));
+  const V v = *(const V*)p;
+  return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+
+// The derivative of a = silu(g) u: du = da silu(g), dg = da u s (1 + g (1 - s)).
+__device__ __forceinline__ void gate_grad(float da, float g, float u, float& dg, float& du) {
+  const float s = sigmoid(g);
+  du = da * silu(g);
+  dg = da * u * (s + silu(g) * (1.0f - s));
+}
+
+// Rows of the padded intermediate buffers are ldi elements apart; one row's
+// valid part is N elements.
+template <typename T, int EPI, int MT, bool BS>
+struct Epilogue {
+  typedef typename Mma<T>::Acc Acc;
+
+  static __device__ __forceinline__ void run(const GemmArgs& g, Acc (&acc)[MT][4], int prob,
+                                             int slice, int m0, int n0, int lane) {
+    const int r = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int m = m0 + mt * 16 + r;
+      if (EPI == kGatedMax) {
+        gated_max(g, acc[mt], m, n0, q);
+        continue;
+      }
+      if (m >= g.M) continue;
+      if constexpr (EPI == kGated) {
+        gated(g, acc[mt], m, n0 + q * 8);
+      } else if constexpr (EPI == kPartGated) {
+        const int64_t at = ((int64_t)slice * g.M + m) * 2 * g.ldp;
+        const int n = n0 + q * 8;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (n + (t & 1) * 4 < g.N)
+            *(Acc*)(reinterpret_cast<char*>(g.part) +
+                    (at + (t >> 1) * g.ldp + n + (t & 1) * 4) * 4) = acc[mt][t];
+      } else if constexpr (EPI == kStore && !BS) {
+        float v[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[t * 4 + i] = acc[mt][t][i];
+        const int n = n0 + q * 16;
+        T* p = (T*)g.out[prob] + (int64_t)m * g.ldo + n;
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 16; i += V) store_run<T, V>(p + i, v + i, g.N - n - i, g.vec);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int n = n0 + (BS ? t * 16 + q * 4 : q * 16 + t * 4);
+          // dg and du rows are read in whole 16-byte chunks: their zeros past N too.
+          if (n < (EPI == kGateGrad ? (g.N + 7) & ~7 : g.N)) tile(g, acc[mt][t], prob, slice, m, n);
+        }
+      }
+    }
+  }
+
+  // Four consecutive n of one m.
+  static __device__ __forceinline__ void tile(const GemmArgs& g, Acc a, int prob, int slice, int m,
+                                              int n) {
+    if constexpr (EPI == kPart) {
+      const int64_t at = (((int64_t)slice * g.nprob + prob) * g.M + m) * g.ldp + n;
+      *(Acc*)(reinterpret_cast<char*>(g.part) + at * 4) = a;  // ldp covers the tail
+    } else if constexpr (EPI == kStore) {
+      const float v[4] = {a[0], a[1], a[2], a[3]};
+      store_run<T, 4>((T*)g.out[prob] + (int64_t)m * g.ldo + n, v, g.N - n, g.vec);
+    } else if constexpr (EPI == kGateGrad) {
+      const int64_t at = (int64_t)m * g.ldi + n;
+      const f32x4 gg = load4((const T*)g.in[0] + at), uu = load4((const T*)g.in[1] + at);
+      float dg[4], du[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) gate_grad(a[i], gg[i], uu[i], dg[i], du[i]);
+      store_run<T, 4>((T*)g.out[0] + at, dg, 4, true);
+      store_run<T, 4>((T*)g.out[1] + at, du, 4, true);
+    } else if constexpr (EPI == kScale) {
+      const float sm = g.row_scale[m];
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = n + i < g.N ? (float)a[i] * sm * g.col_scale[0][n + i] : 0.0f;
+      const int64_t at = (int64_t)m * g.ldo + n;
+      if (g.out_dtype == WR_F32)
+        store_run<float, 4>((float*)g.out[0] + at, v, g.N - n, g.vec);
+      else if (g.out_dtype == WR_F16)
+        store_run<f16, 4>((f16*)g.out[0] + at, v, g.N - n, g.vec);
+      else
+        store_run<bf16, 4>((bf16*)g.out[0] + at, v, g.N - n, g.vec);
+    }
+  }
+
+  // 8 gate and 8 up sums of the same n (acc[0..1] and acc[2..3]).  The buffers'
+  // rows are padded to ldi (a multiple of 64), so whole vectors are stored.
+  static __device__ __forceinline__ void gated(const GemmArgs& g, const Acc (&acc)[4], int m,
+                                               int n) {
+    if (n >= g.N) return;
+    float a[8], gg[8], uu[8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        gg[t * 4 + i] = acc[t][i];
+        uu[t * 4 + i] = acc[t + 2][i];
+        a[t * 4 + i] = silu(acc[t][i]) * acc[t + 2][i];
+      }
+    const int64_t at = (int64_t)m * g.ldi + n;
+    constexpr int V = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;
+#pragma unroll
+    for (int i = 0; i < 8; i += V) {
+      store_run<T, V>((T*)g.out[0] + at + i, a + i, V, true);
+      if (g.out[1] != nullptr) {
+        store_run<T, V>((T*)g.out[1] + at + i, gg + i, V, true);
+        store_run<T, V>((T*)g.out[2] + at + i, uu + i, V, true);
+      }
+    }
+  }
+
+  // int8: a = silu(g) u in fp32 with its row maxima of |a| (as fp32 bits: the
+  // maximum of non-negative floats is that of their bits, in any order).
+  static __device__ __forceinline__ void gated_max(const GemmArgs& g, const Acc (&acc)[4], int m,
+                                                   int n0, int q) {
+    const int n = n0 + q * 8;
+    unsigned mx = 0;
+    if (m < g.M && n < g.N) {
+      const float sm = g.row_scale[m];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = n + t * 4 + i;
+          v[i] = 0.0f;
+          if (c < g.N) {
+            const float gg = (float)acc[t][i] * sm * g.col_scale[0][c];
+            v[i] = silu(gg) * ((float)acc[t + 2][i] * sm * g.col_scale[1][c]);
+          }
+          mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
+        }
+        store_run<float, 4>((float*)g.out[0] + (int64_t)m * g.ldi + n + t * 4, v, 4, true);
+      }
+    }
+    mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
+    mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
+    if (q == 0 && m < g.M) atomicMax(g.row_max + m, mx);
+  }
+};
+
+// Bytes of a row up to the end of its last 16-byte chunk (rows are padded to whole chunks).
+__device__ __forceinline__ int64_t chunked(int64_t bytes) { return (bytes + 15) & ~(int64_t)15; }
+
+// ---- the kernel -------------------------------------------------------------
+template <typename T, int WM, int WN, int MT, bool AS, bool BS, int EPI>
+__global__ __launch_bounds__(WM* WN * 64) void k_dense(GemmArgs g) {
+  constexpr bool GATED = EPI == kGated || EPI == kGatedMax || EPI == kPartGated;
+  constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * 64;
+  constexpr int ABYTES = BM * kStepBytes, BBYTES = BN * kStepBytes;
+  constexpr int ES = sizeof(T), KB = kStepBytes / ES;
+  typedef typename Mma<T>::Acc Acc;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * (ABYTES + BBYTES)];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  // Block -> (slice, problem, tile).  Consecutive blocks go to the 8 XCDs in
+  // turn, so each XCD takes one run of the tile order; within it 8 m tiles
+  // advance together along n, for both operands' reuse in the XCD's L2.
+  const TileId id = tile_of(g, (int)blockIdx.x, (int)gridDim.x);
+  const int m0 = id.m * BM, n0 = id.n * (GATED ? BN / 2 : BN);
+  const int steps = (g.K + KB - 1) / KB, total = steps * g.nseg;
+  const int per = (total + g.slices - 1) / g.slices;
+  const int s0 = id.slice * per, s1 = min(total, s0 + per);
+
+  TileCopy<T, BM, NW, AS, false, false> ca;
+  TileCopy<T, BN, NW, BS, true, GATED> cb;
+  ca.init(wave, lane, g.lda, AS ? g.M - m0 : 0);
+  cb.init(wave, lane, g.ldb, BS ? g.N - n0 : 0);
+  Frag<T, BM, MT, AS, false> fa;
+  Frag<T, BN, 4, BS, true> fb;
+  fa.init(wm * MT, lane);
+  fb.init(wn * 4, lane);
+
+  auto copy = [&](int step, char* lds) {
+    const int seg = step >= steps ? 1 : 0;
+    const int k = (step - seg * steps) * KB;
+    {
+      const char* p = g.a[g.nprob > 1 ? id.prob : seg];
+      const int64_t off = AS ? k * g.lda + (int64_t)m0 * ES : m0 * g.lda + (int64_t)k * ES;
+      const int64_t all = AS ? (g.K - 1) * g.lda + chunked((int64_t)g.M * ES)
+                             : (g.M - 1) * g.lda + chunked((int64_t)g.K * ES);
+      ca.issue(lds, p + off, all - off, g.K - k, wave, lane);
+    }
+    {
+      const char* p = g.b[GATED ? (wave & 1) : seg];
+      const int64_t off = BS ? k * g.ldb + (int64_t)n0 * ES : n0 * g.ldb + (int64_t)k * ES;
+      const int64_t all = BS ? (g.K - 1) * g.ldb + chunked((int64_t)g.N * ES)
+                             : (g.N - 1) * g.ldb + chunked((int64_t)g.K * ES);
+      cb.issue(lds + ABYTES, p + off, all - off, g.K - k, wave, lane);
+    }
+  };
+
+  Acc acc[MT][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[i][t] = Acc{};
+
+  if (s0 < s1) copy(s0, smem);
+  __syncthreads();
+  for (int s = s0; s < s1; ++s) {
+    char* cur = smem + ((s - s0) & 1) * (ABYTES + BBYTES);
+    if (s + 1 < s1) copy(s + 1, smem + ((s + 1 - s0) & 1) * (ABYTES + BBYTES));
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      u32x4 b[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) b[t] = fb.get(cur + ABYTES, t, kk);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const u32x4 a = fa.get(cur, i, kk);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[i][t] = Mma<T>::go(b[t], a, acc[i][t]);
+      }
+    }
+    __syncthreads();
+  }
+  Epilogue<T, EPI, MT, BS>::run(g, acc, id.prob, id.slice, m0 + wm * MT * 16,
+                                n0 + wn * (GATED ? 32 : 64), lane);
+}
+
+// The epilogue of a product split over K: the slices' sums added in order, then as
+// in k_dense.  One thread per 4 columns; blockIdx.y counts rows (and problems).
+template <typename T, int EPI>
+__global__ __launch_bounds__(256) void k_dense_join(GemmArgs g) {
+  typedef typename Mma<T>::Acc Acc;
+  constexpr bool GATED = EPI == kGated || EPI == kGatedMax;
+  const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+  const int limit = EPI == kStore || EPI == kScale ? g.N : (g.N + 7) & ~7;
+  for (int64_t row = blockIdx.y; row < (int64_t)g.M * g.nprob; row += gridDim.y) {
+    const int prob = (int)(row / g.M), m = (int)(row % g.M);
+    const int64_t ld = GATED ? 2 * g.ldp : g.ldp;
+    const Acc* p = (const Acc*)g.part + (row * ld + n) / 4;
+    const int64_t step = (int64_t)g.nprob * g.M * ld / 4;
+    Acc s = Acc{}, u = Acc{};
+    if (n < g.N) {
+      for (int i = 0; i < g.slices; ++i) {
+        s += p[i * step];
+        if (GATED) u += p[i * step + g.ldp / 4];
+      }
+    }
+    if constexpr (EPI == kGated) {
+      if (n >= limit) continue;
+      float a[4], gg[4], uu[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        gg[i] = s[i];
+        uu[i] = u[i];
+        a[i] = silu(s[i]) * u[i];
+      }
+      const int64_t at = (int64_t)m * g.ldi + n;
+      store_run<T, 4>((T*)g.out[0] + at, a, 4, true);
+      if (g.out[1] != nullptr) {
+        store_run<T, 4>((T*)g.out[1] + at, gg, 4, true);
+        store_run<T, 4>((T*)g.out[2] + at, uu, 4, true);
+      }
+    } else if constexpr (EPI == kGatedMax) {
+      unsigned mx = 0;
+      if (n < limit) {
+        float v[4];
+        const float sm = g.row_scale[m];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = 0.0f;
+          if (n + i < g.N) {
+            const float gg = (float)s[i] * sm * g.col_scale[0][n + i];
+            v[i] = silu(gg) * ((float)u[i] * sm * g.col_scale[1][n + i]);
+          }
+          mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
+        }
+        store_run<float, 4>((float*)g.out[0] + (int64_t)m * g.ldi + n, v, 4, true);
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) mx = max(mx, (unsigned)__shfl_xor((int)mx, d));
+      if ((threadIdx.x & 63) == 0) atomicMax(g.row_max + m, mx);
+    } else {
+      if (n < limit) Epilogue<T, EPI, 1, true>::tile(g, s, prob, 0, m, n);
+    }
+  }
+}
+
+// ---- launching --------------------------------------------------------------
+template <typename T, int WM, int WN, int MT, bool AS, bool BS, int EPI>
+hipError_t launch_tile(const GemmArgs& g, hipStream_t s) {
+  const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.nprob * g.slices;
+  k_dense<T, WM, WN, MT, AS, BS, EPI><<<(unsigned)blocks, WM * WN * 64, 0, s>>>(g);
+  return hipGetLastError();
+}
+
+template <typename T, bool AS, bool BS, int EPI>
+hipError_t launch_shape(const GemmArgs& g, int shape, hipStream_t s) {
+  switch (shape) {
+    case kTile256: return launch_tile<T, 2, 4, 8, AS, BS, EPI>(g, s);
+    case kTile128: return launch_tile<T, 2, 2, 4, AS, BS, EPI>(g, s);
+    default: return launch_tile<T, 1, 4, 4, AS, BS, EPI>(g, s);
+  }
+}
+
+// EPI of the whole product; SPLIT the epilogue of its slices.
+template <typename T, bool AS, bool BS, int EPI, int SPLIT>
+hipError_t launch_epi(const GemmArgs& g, int shape, hipStream_t s) {
+  if (g.slices == 1) return launch_shape<T, AS, BS, EPI>(g, shape, s);
+  const hipError_t e = launch_shape<T, AS, BS, SPLIT>(g, shape, s);
+  if (e != hipSuccess) return e;
+  const int64_t rows = (int64_t)g.M * g.nprob;
+  const dim3 grid((g.N + 1023) / 1024, (unsigned)(rows < 65535 ? rows : 65535));
+  k_dense_join<T, EPI><<<grid, 256, 0, s>>>(g);
+  return hipGetLastError();
+}
+
+// The products of a floating-point type.
+template <typename T>
+hipError_t launch_float(const GemmArgs& g, int shape, int form, hipStream_t s) {
+  switch (form) {
+    case kFormGated: return launch_epi<T, false, false, kGated, kPartGated>(g, shape, s);
+    case kFormKcKc: return launch_epi<T, false, false, kStore, kPart>(g, shape, s);
+    case kFormGateGrad: return launch_epi<T, false, true, kGateGrad, kPart>(g, shape, s);
+    case kFormKcKs: return launch_epi<T, false, true, kStore, kPart>(g, shape, s);
+    default: return launch_epi<T, true, true, kStore, kPart>(g, shape, s);
+  }
+}
+
+}  // namespace ffn
+}  // namespace wr

@@ -20,10 +20,12 @@ import torch
 import torch.nn as nn
 
 from .functional import (MAX_EXPERTS, MAX_TOPK, WEIGHT_DTYPES, _pack_expert_weights,
-                         batched_fused_moe, expert_layout, fused_moe, gate_topk, naive_moe,
-                         quantize_fp8, quantize_mxfp4, weight_layout)
+                         batched_fused_moe, expert_layout, fused_moe, gate_topk, gated_ffn,
+                         gated_ffn_int8, int8_matmul, naive_moe, quantize_fp8, quantize_int8,
+                         quantize_mxfp4, weight_layout)
 
-__all__ = ["MoELayer", "fused_moe", "naive_moe", "batched_fused_moe", "gate_topk",
+__all__ = ["MoELayer", "GatedFFN", "Int8GatedFFN", "gated_ffn", "gated_ffn_int8", "quantize_int8",
+           "int8_matmul", "fused_moe", "naive_moe", "batched_fused_moe", "gate_topk",
            "expert_layout", "weight_layout", "quantize_fp8", "quantize_mxfp4",
            "_pack_expert_weights"]
 
@@ -128,3 +130,56 @@ class MoELayer(nn.Module):
                                      self.hidden_dim, self.intermediate_dim, self.top_k,
                                      self.renormalize)
         raise ValueError(f"Input must be 1D or 2D, got shape {x.shape}")
+
+
+class GatedFFN(nn.Module):
+    """Dense SwiGLU FFN, or the shared expert of an MoE layer: the same three
+    matrices as one expert of ``MoELayer``, applied to every token and
+    differentiable (``functional.gated_ffn``).
+
+    Args:
+        hidden_dim: hidden state dimension.
+        intermediate_dim: intermediate dimension.
+        dtype: dtype of the parameters, the tokens and the output
+            (torch.float32, torch.float16 or torch.bfloat16).
+    """
+
+    def __init__(self, hidden_dim: int, intermediate_dim: int,
+                 dtype: torch.dtype = torch.float32) -> None:
+        super().__init__()
+        if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+        self.hidden_dim = hidden_dim
+        self.intermediate_dim = intermediate_dim
+        self.gate_proj = nn.Parameter(torch.empty(intermediate_dim, hidden_dim, dtype=dtype))
+        self.up_proj = nn.Parameter(torch.empty(intermediate_dim, hidden_dim, dtype=dtype))
+        self.down_proj = nn.Parameter(torch.empty(hidden_dim, intermediate_dim, dtype=dtype))
+        for p in self.parameters():
+            nn.init.normal_(p, std=0.02)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """[..., hidden_dim] -> the same shape and dtype."""
+        return gated_ffn(x.contiguous(), self.gate_proj, self.up_proj, self.down_proj)
+
+    def quantized(self) -> "Int8GatedFFN":
+        """The int8 serving form of the present parameters (on the GPU)."""
+        return Int8GatedFFN(self)
+
+
+class Int8GatedFFN(nn.Module):
+    """A GatedFFN's weights in int8 with an fp32 scale per output channel, held
+    as buffers (``functional.gated_ffn_int8``; inference only)."""
+
+    def __init__(self, ffn: GatedFFN) -> None:
+        super().__init__()
+        self.hidden_dim = ffn.hidden_dim
+        self.intermediate_dim = ffn.intermediate_dim
+        for name in ("gate", "up", "down"):
+            codes, scales = quantize_int8(getattr(ffn, f"{name}_proj").detach())
+            self.register_buffer(f"{name}_codes", codes)
+            self.register_buffer(f"{name}_scales", scales)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """[..., hidden_dim] -> the same shape and dtype."""
+        return gated_ffn_int8(x.contiguous(), self.gate_codes, self.gate_scales, self.up_codes,
+                              self.up_scales, self.down_codes, self.down_scales)

@@ -30,6 +30,7 @@ WR_EINVAL_KIND = 9
 WR_EINVAL_BLOCK = 10
 WR_ETIMEOUT = 11
 WR_EINVAL_SCRATCH = 12
+WR_EINVAL_ALIGN = 13
 WR_NOALLOC_SCRATCH_BYTES = 1 << 20
 WR_EHIP = 100
 
@@ -42,6 +43,10 @@ WR_MXFP4 = 4
 WR_KIND_FUSED = 0
 WR_KIND_BATCHED = 1
 WR_KIND_NAIVE = 2
+
+# include/wr_ffn.h
+WR_FFN_MAX_DIM = 1 << 20
+WR_INT8_MAX_K = 131071
 
 
 class WrOffsets(ctypes.Structure):
@@ -83,6 +88,27 @@ class WrMoeArgs(ctypes.Structure):
     ]
 
 
+class WrFfnArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "x", "w_gate", "w_up", "w_down", "out", "saved_gate", "saved_up", "saved_act", "dout", "dx",
+        "dw_gate", "dw_up", "dw_down")] + [
+        (n, ctypes.c_int32) for n in ("dtype", "batch_size", "hidden_dim", "intermediate_dim")] + [
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class WrInt8Args(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "x_scale", "w", "w_scale", "out")] + [
+        (n, ctypes.c_int32) for n in ("out_dtype", "rows", "out_features", "in_features")] + [
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class WrFfnInt8Args(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "x", "w_gate", "s_gate", "w_up", "s_up", "w_down", "s_down", "out")] + [
+        (n, ctypes.c_int32) for n in ("dtype", "batch_size", "hidden_dim", "intermediate_dim")] + [
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -115,6 +141,20 @@ def lib() -> ctypes.CDLL:
         l.wr_fused_moe_status.restype = ctypes.c_int
         l.wr_fused_moe_expired.argtypes = [ctypes.c_int]
         l.wr_fused_moe_expired.restype = ctypes.c_int
+        # include/wr_ffn.h
+        l.wr_ffn_saved_row.argtypes = [ctypes.c_int]
+        l.wr_ffn_saved_row.restype = ctypes.c_int64
+        for name, n in (("wr_ffn_workspace_bytes", 5), ("wr_int8_workspace_bytes", 3),
+                        ("wr_ffn_int8_workspace_bytes", 3)):
+            getattr(l, name).argtypes = [ctypes.c_int] * n
+            getattr(l, name).restype = ctypes.c_size_t
+        for name, args in (("wr_ffn_forward", WrFfnArgs), ("wr_ffn_backward", WrFfnArgs),
+                           ("wr_int8_matmul", WrInt8Args), ("wr_ffn_int8", WrFfnInt8Args)):
+            getattr(l, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+            getattr(l, name).restype = ctypes.c_int
+        l.wr_quantize_int8.argtypes = ([ctypes.c_void_p] + [ctypes.c_int] * 3 +
+                                       [ctypes.c_void_p] * 3)
+        l.wr_quantize_int8.restype = ctypes.c_int
         # include/wr_timeline.h (measurement hook)
         l.wr_timeline_read.argtypes = [ctypes.POINTER(ctypes.c_uint64), ctypes.c_int64,
                                        ctypes.c_void_p]

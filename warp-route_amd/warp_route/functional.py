@@ -20,10 +20,16 @@ E2M1 codes per byte plus an E8M0 scale per 32 elements), see
 dtype.  Work runs on the current
 HIP stream without a device synchronisation.  There is no CPU fallback: the
 ops raise if the HIP extension is missing.
+
+Beside the routed layer stand the operators of a dense FFN (a model's dense
+layers, or the shared expert of an MoE layer), which the reference does not
+have: ``gated_ffn``, differentiable, in float32, float16 or bfloat16, and its
+int8 serving form, ``quantize_int8``, ``int8_matmul`` and ``gated_ffn_int8``.
 """
 from __future__ import annotations
 
 import functools
+import math
 from typing import List, Optional, Tuple
 
 import torch
@@ -382,3 +388,91 @@ def gate_topk(
     weight order, ties to the lower index."""
     _C = _load_extension()
     return _C.gate_topk(x, gate_w, num_experts, hidden_dim, top_k, renormalize)
+
+
+class _GatedFFN(torch.autograd.Function):
+    """gated_ffn with its backward pass.  Keeps g = x w_gate^T, u = x w_up^T and
+    silu(g) u in x's dtype (rows padded to 64 elements) for the gradients."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down):
+        y, g, u, a = _load_extension().gated_ffn_forward(x, w_gate, w_up, w_down, True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, g, u, a)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return tuple(_load_extension().gated_ffn_backward(
+            dy.contiguous(), *ctx.saved_tensors, list(ctx.needs_input_grad)))
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x [..., n] as [rows, n]."""
+    if x.dim() == 0:
+        raise ValueError("x must have at least one dimension")
+    return x if x.dim() == 2 else x.reshape(-1 if x.numel() else math.prod(x.shape[:-1]),
+                                            x.shape[-1])
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+              w_down: torch.Tensor) -> torch.Tensor:
+    """Dense gated FFN: (silu(x w_gate^T) * (x w_up^T)) w_down^T.
+
+    Args:
+        x: tokens [..., hidden_dim], any number of them, float32, float16 or
+            bfloat16, contiguous, on the GPU.
+        w_gate, w_up: [intermediate_dim, hidden_dim] in x's dtype.
+        w_down: [hidden_dim, intermediate_dim] in x's dtype.
+
+    Returns x's shape and dtype.  Sums are fp32; the activations between the
+    two products are rounded to x's dtype, as are the values kept for the
+    backward pass (three buffers of x's rows times intermediate_dim, only when
+    a gradient is needed).  Differentiable once with respect to all four
+    arguments; gradients that are not needed are not computed.
+
+    Forward and backward launch kernels on the current stream only and may be
+    captured in a HIP graph.  As for any torch operator, no eager graph of the
+    same leaf tensors may be alive when a backward pass is captured.
+    """
+    rows = _rows(x)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
+        y = _GatedFFN.apply(rows, w_gate, w_up, w_down)
+    else:
+        y = _load_extension().gated_ffn_forward(rows, w_gate, w_up, w_down, False)[0]
+    return y if x.dim() == 2 else y.reshape(x.shape)
+
+
+def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of x [..., n] in int8 with one fp32 scale per row (token,
+    or output channel of a weight): scale = max|row| / 127, codes = 127 x /
+    max|row| rounded to nearest, ties to even, exactly.  A zero row gets codes
+    0 and scale 1; a row with a non-finite value gets codes 0 and scale NaN, so
+    that only what is computed from it is NaN.  Codes have x's shape, scales
+    x's shape without its last dimension."""
+    q, s = _load_extension().quantize_int8(_rows(x))
+    return q.reshape(x.shape), s.reshape(x.shape[:-1])
+
+
+def int8_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """out[..., n] = (sum_k x[..., k] w[n, k]) * x_scale[...] * w_scale[n] for
+    int8 codes x [..., K] and w [N, K] (K at most 131071) with fp32 scales per
+    token and per output channel (``quantize_int8``).  The sum is exact; it is
+    scaled in fp32 and rounded once to out_dtype (float32, float16 or
+    bfloat16)."""
+    out = _load_extension().int8_matmul(_rows(x), x_scale.reshape(-1), w, w_scale, out_dtype)
+    return out if x.dim() == 2 else out.reshape(*x.shape[:-1], out.shape[-1])
+
+
+def gated_ffn_int8(x: torch.Tensor, w_gate: torch.Tensor, s_gate: torch.Tensor,
+                   w_up: torch.Tensor, s_up: torch.Tensor, w_down: torch.Tensor,
+                   s_down: torch.Tensor) -> torch.Tensor:
+    """``gated_ffn`` on int8 weights (codes and scales per output channel, as
+    ``quantize_int8`` of each matrix gives): x is quantised per token, the
+    activations silu(g) * u are computed in fp32 from the exact int8 sums and
+    quantised per token too.  x is float32, float16 or bfloat16; returns x's
+    shape and dtype.  Inference only."""
+    y = _load_extension().gated_ffn_int8(_rows(x.detach()), w_gate, s_gate, w_up, s_up, w_down,
+                                         s_down)
+    return y if x.dim() == 2 else y.reshape(x.shape)

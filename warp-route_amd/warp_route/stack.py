@@ -14,7 +14,7 @@ pool while capturing), record no memset nodes, and never synchronise.
 """
 from __future__ import annotations
 
-from typing import List, Sequence, Tuple
+from typing import Callable, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -27,11 +27,14 @@ class MoEStack:
     """Layers l = 0..L-1, each a (gate_w [E, h] fp32, packed expert buffer)
     pair of the same shape.  One step maps x ([h] for one token, [B, h] for a
     batch) to h_L with h_0 = x and h_{l+1} = h_l + moe_l(h_l) (residual=True)
-    or h_{l+1} = moe_l(h_l)."""
+    or h_{l+1} = moe_l(h_l).  With ``shared``, one callable (or None) per layer
+    from the tokens to the same shape and dtype, such as ``GatedFFN`` or
+    ``Int8GatedFFN``, layer l's shared expert adds shared_l(h_l) to moe_l(h_l)."""
 
     def __init__(self, layers: Sequence[Tuple[torch.Tensor, torch.Tensor]], num_experts: int,
                  hidden_dim: int, intermediate_dim: int, top_k: int,
-                 renormalize: bool = False, residual: bool = True) -> None:
+                 renormalize: bool = False, residual: bool = True,
+                 shared: Optional[Sequence[Optional[Callable]]] = None) -> None:
         if len(layers) == 0:
             raise ValueError("MoEStack needs at least one layer")
         for i, (gw, buf) in enumerate(layers):
@@ -40,6 +43,10 @@ class MoEStack:
                                  f"got {tuple(gw.shape)}")
             if buf.device != gw.device:
                 raise ValueError(f"layer {i}: gate_w and weight_buf on different devices")
+        if shared is not None and len(shared) != len(layers):
+            raise ValueError(f"shared must hold one entry per layer ({len(layers)}), "
+                             f"got {len(shared)}")
+        self.shared = list(shared) if shared is not None else [None] * len(layers)
         self.layers: List[Tuple[torch.Tensor, torch.Tensor]] = list(layers)
         self.num_experts = num_experts
         self.hidden_dim = hidden_dim
@@ -60,8 +67,11 @@ class MoEStack:
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """One decode step, launched op by op."""
         h = x.contiguous()
-        for gw, buf in self.layers:
+        for (gw, buf), shared in zip(self.layers, self.shared):
             y = self._moe(h, gw, buf)
+            if shared is not None:
+                with torch.no_grad():  # a decode step, as the routed layer
+                    y = y + shared(h)
             h = h + y if self.residual else y
         return h
 
