@@ -12,8 +12,9 @@
  * and for a gradient dy of y, with da = dy Wd:
  *   du = da g s,  dg = da u s (1 + g (1 - s))
  *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T a
- * Sums are fp32.  a, g, u, dg and du are rounded to the call's dtype where
- * they are stored between products.
+ * Sums are fp32.  a, dg and du are rounded to the call's dtype, in which the
+ * matrix cores read them; g and u are kept in fp32, so that the gradients
+ * see one rounding before their last product, as y does.
  *
  * Matrices are row-major and contiguous; pointers are 16-byte aligned.
  * A call may be recorded into a HIP graph.
@@ -38,9 +39,9 @@ typedef struct wr_ffn_args {
   const void *w_up;     /* [I, h]                                               */
   const void *w_down;   /* [h, I]                                               */
   void *out;            /* forward: y [T, h]                                    */
-  void *saved_gate;     /* g, u and a, [T, wr_ffn_saved_row(I)] each.  Forward: */
-  void *saved_up;       /*   written when all three are given, all NULL: not    */
-  void *saved_act;      /*   kept.  Backward: as the forward call wrote them.   */
+  float *saved_gate;    /* g, u (fp32) and a (dtype), [T, wr_ffn_saved_row(I)]  */
+  float *saved_up;      /*   each.  Forward: written when all three are given,  */
+  void *saved_act;      /*   all NULL: not kept.  Backward: as forward wrote.   */
   const void *dout;     /* backward: dy [T, h]                                  */
   void *dx;             /* backward: gradients, each optional (NULL: not       */
   void *dw_gate;        /*   computed)                                          */

@@ -56,9 +56,7 @@ def ffn_grads(x, wg, wu, wd, dy):
     dt = x.dtype
     g, uu, a, eg, eu, ea = gate_parts(x, wg, wu, dt)
     x, wg, wu, wd, dy = (t.double() for t in (x, wg, wu, wd, dy))
-    # g, u and a are kept in x's dtype
-    eg = eg + u(dt) * (g.abs() + eg) + step(dt)
-    eu = eu + u(dt) * (uu.abs() + eu) + step(dt)
+    # a is kept in x's dtype, g and u in fp32
     ea = ea + u(dt) * (a.abs() + ea) + step(dt)
     s = torch.sigmoid(g)
     silu, f = g * s, s * (1 + g * (1 - s))  # f = silu', |f| <= 1.1, |f'| <= 0.5

@@ -381,10 +381,11 @@ std::vector<torch::Tensor> gated_ffn_forward(torch::Tensor x, torch::Tensor w_ga
   wr_ffn_args a = ffn_args(x, w_gate, w_up, w_down);
   if (keep) {
     for (int i = 0; i < 3; ++i)
-      out.push_back(torch::empty({x.size(0), wr_ffn_saved_row(a.intermediate_dim)}, x.options()));
+      out.push_back(torch::empty({x.size(0), wr_ffn_saved_row(a.intermediate_dim)},
+                                 i < 2 ? x.options().dtype(torch::kFloat32) : x.options()));
     if (x.size(0) > 0) {
-      a.saved_gate = out[1].data_ptr();
-      a.saved_up = out[2].data_ptr();
+      a.saved_gate = out[1].data_ptr<float>();
+      a.saved_up = out[2].data_ptr<float>();
       a.saved_act = out[3].data_ptr();
     }
   }
@@ -408,8 +409,8 @@ std::vector<std::optional<torch::Tensor>> gated_ffn_backward(
   const torch::Device dev = x.device();
   check_operand(dy, "dy", x.scalar_type(), dev, x.sizes());
   const int64_t row = wr_ffn_saved_row((int)w_gate.size(0));
-  check_operand(g, "g", x.scalar_type(), dev, {x.size(0), row});
-  check_operand(u, "u", x.scalar_type(), dev, {x.size(0), row});
+  check_operand(g, "g", torch::kFloat32, dev, {x.size(0), row});
+  check_operand(u, "u", torch::kFloat32, dev, {x.size(0), row});
   check_operand(act, "a", x.scalar_type(), dev, {x.size(0), row});
   TORCH_CHECK(need.size() == 4, "need must hold 4 truth values, got ", need.size());
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
@@ -434,8 +435,8 @@ std::vector<std::optional<torch::Tensor>> gated_ffn_backward(
   }
   if (!any) return out;
   a.dout = dy.data_ptr();
-  a.saved_gate = g.data_ptr();
-  a.saved_up = u.data_ptr();
+  a.saved_gate = g.data_ptr<float>();
+  a.saved_up = u.data_ptr<float>();
   a.saved_act = act.data_ptr();
   torch::Tensor ws = scratch(
       wr_ffn_workspace_bytes(1, a.dtype, a.hidden_dim, a.intermediate_dim, a.batch_size), dev);

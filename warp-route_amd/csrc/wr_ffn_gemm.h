@@ -246,13 +246,6 @@ __device__ __forceinline__ void store_run(T* p, const float* v, int left, bool v
   }
 }
 
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* p) {
-  typedef T V __attribute__((ext_vector_type(4)));
-  const V v = *(const V*)p;
-  return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
-}
-
 // The derivative of a = silu(g) u: du = da silu(g), dg = da u s (1 + g (1 - s)).
 __device__ __forceinline__ void gate_grad(float da, float g, float u, float& dg, float& du) {
   const float s = sigmoid(g);
@@ -320,7 +313,8 @@ struct Epilogue {
       store_run<T, 4>((T*)g.out[prob] + (int64_t)m * g.ldo + n, v, g.N - n, g.vec);
     } else if constexpr (EPI == kGateGrad) {
       const int64_t at = (int64_t)m * g.ldi + n;
-      const f32x4 gg = load4((const T*)g.in[0] + at), uu = load4((const T*)g.in[1] + at);
+      const f32x4 gg = *(const f32x4*)((const float*)g.in[0] + at);
+      const f32x4 uu = *(const f32x4*)((const float*)g.in[1] + at);
       float dg[4], du[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) gate_grad(a[i], gg[i], uu[i], dg[i], du[i]);
@@ -359,11 +353,12 @@ struct Epilogue {
     const int64_t at = (int64_t)m * g.ldi + n;
     constexpr int V = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;
 #pragma unroll
-    for (int i = 0; i < 8; i += V) {
-      store_run<T, V>((T*)g.out[0] + at + i, a + i, V, true);
-      if (g.out[1] != nullptr) {
-        store_run<T, V>((T*)g.out[1] + at + i, gg + i, V, true);
-        store_run<T, V>((T*)g.out[2] + at + i, uu + i, V, true);
+    for (int i = 0; i < 8; i += V) store_run<T, V>((T*)g.out[0] + at + i, a + i, V, true);
+    if (g.out[1] != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        store_run<float, 4>((float*)g.out[1] + at + i, gg + i, 4, true);
+        store_run<float, 4>((float*)g.out[2] + at + i, uu + i, 4, true);
       }
     }
   }
@@ -513,8 +508,8 @@ __global__ __launch_bounds__(256) void k_dense_join(GemmArgs g) {
       const int64_t at = (int64_t)m * g.ldi + n;
       store_run<T, 4>((T*)g.out[0] + at, a, 4, true);
       if (g.out[1] != nullptr) {
-        store_run<T, 4>((T*)g.out[1] + at, gg, 4, true);
-        store_run<T, 4>((T*)g.out[2] + at, uu, 4, true);
+        store_run<float, 4>((float*)g.out[1] + at, gg, 4, true);
+        store_run<float, 4>((float*)g.out[2] + at, uu, 4, true);
       }
     } else if constexpr (EPI == kGatedMax) {
       unsigned mx = 0;

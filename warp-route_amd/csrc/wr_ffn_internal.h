@@ -11,8 +11,8 @@ namespace ffn {
 
 enum Epi {
   kStore,      // out[prob][m][n]
-  kGated,      // out[0] = silu(g) u, and out[1] = g, out[2] = u when set; ldi rows
-  kGateGrad,   // out[0] = dg, out[1] = du from in[0] = g, in[1] = u; ldi rows
+  kGated,      // out[0] = silu(g) u, and out[1] = g, out[2] = u (fp32) when set; ldi rows
+  kGateGrad,   // out[0] = dg, out[1] = du from in[0] = g, in[1] = u (fp32); ldi rows
   kScale,      // int8: out[0] = sum * row_scale[m] * col_scale[0][n], of out_dtype
   kGatedMax,   // int8: out[0] = silu(g) u in fp32, ldi rows; row_max[m] = max |.|
   kPart,       // part[slice][prob][m][n], rows ldp

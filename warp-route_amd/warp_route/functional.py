@@ -392,7 +392,8 @@ def gate_topk(
 
 class _GatedFFN(torch.autograd.Function):
     """gated_ffn with its backward pass.  Keeps g = x w_gate^T, u = x w_up^T and
-    silu(g) u in x's dtype (rows padded to 64 elements) for the gradients."""
+    silu(g) u (fp32, fp32 and x's dtype; rows padded to 64 elements) for the
+    gradients."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down):
@@ -426,9 +427,9 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
         w_down: [hidden_dim, intermediate_dim] in x's dtype.
 
     Returns x's shape and dtype.  Sums are fp32; the activations between the
-    two products are rounded to x's dtype, as are the values kept for the
-    backward pass (three buffers of x's rows times intermediate_dim, only when
-    a gradient is needed).  Differentiable once with respect to all four
+    two products are rounded to x's dtype.  When a gradient is needed, three
+    buffers of x's rows times intermediate_dim are kept for it: both
+    pre-activations in fp32 and the activations in x's dtype.  Differentiable once with respect to all four
     arguments; gradients that are not needed are not computed.
 
     Forward and backward launch kernels on the current stream only and may be
