@@ -20,7 +20,7 @@
 // last element, so rows past the end arrive as zeros without a branch; K
 // tails and column tails give their lanes an offset behind the descriptor.
 //
-// A wave owns MT x 4 tiles of 16 x 16.  B is the MFMA's first operand, so a
+// A wave owns MT x 4 G tiles of 16 x 16.  B is the MFMA's first operand, so a
 // lane's four accumulators are four consecutive n of one m.  For KC B the
 // LDS rows of a wave's 64 n are dealt to the MFMA rows so that a lane's 4
 // tiles together hold 16 consecutive n (gated: 8 of gate and the same 8 of
@@ -53,45 +53,59 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kStepBytes = 128;  // bytes of K per step
 constexpr unsigned kOutside = 0x80000000u;  // offset behind every descriptor
 
-// ---- one 16 x 16 tile product over 64 bytes of K ---------------------------
+// ---- 16 x 16 tile products over 64 bytes of K --------------------------------
+// The 16-bit and int8 instructions are written as assembly with the sums tied to
+// accumulation registers: the compiler's own register allocation moves the sums of
+// a 128 x 128 wave tile (all 256 accumulation registers) between registers in the
+// loop.  The waits its hazard pass would add are held by construction: fragments
+// come from LDS reads alone (no vector instruction writes them), equal sums are at
+// least NT products apart, and settle() stands between the sums' first and last
+// use and any other instruction on them.
 template <typename T>
 struct Mma;
 template <>
 struct Mma<bf16> {
   typedef f32x4 Acc;
-  static __device__ __forceinline__ Acc go(u32x4 a, u32x4 b, Acc c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
 };
 template <>
 struct Mma<f16> {
   typedef f32x4 Acc;
-  static __device__ __forceinline__ Acc go(u32x4 a, u32x4 b, Acc c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
-                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
 };
 template <>
 struct Mma<int8_t> {
   typedef i32x4 Acc;
-  static __device__ __forceinline__ Acc go(u32x4 a, u32x4 b, Acc c) {
-    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a),
-                                                 __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+  static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
+    asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
 };
 // fp32: lane group q holds k = 4 q .. 4 q + 3, one element per MFMA.
 template <>
 struct Mma<float> {
   typedef f32x4 Acc;
-  static __device__ __forceinline__ Acc go(u32x4 a, u32x4 b, Acc c) {
+  static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
     const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-    return c;
   }
 };
+
+// Orders all accumulators' values between the assembly products and other instructions,
+// with the wait states of the longest product (18) in between.
+template <typename Acc, int N>
+__device__ __forceinline__ void settle(Acc (&acc)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+a"(acc[i]));
+  asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+a"(acc[i]));
+}
 
 // ---- copying one operand's K step into LDS ---------------------------------
 // Swizzle keys: KC tiles are [row][128 bytes], KS tiles [k][ROWS elements].
@@ -111,11 +125,10 @@ __device__ __forceinline__ int ks_key(int k) {  // xor of the 32- (64-) byte chu
 template <typename T, int ROWS, int NW, bool KS, bool NSIDE, bool GATED>
 struct TileCopy {
   static constexpr int ES = sizeof(T);
-  static constexpr int kBytes = ROWS * kStepBytes;
-  static constexpr int kCopies = kBytes / 1024;
-  static constexpr int PER = (kCopies + NW - 1) / NW;
-  static constexpr int kStep = kStepBytes / ES;     // K elements per step
-  static constexpr int EPC = 16 / ES;               // elements per chunk
+  static constexpr int kCopies = ROWS * kStepBytes / 1024;
+  static constexpr int PER = kCopies / NW;
+  static_assert(kCopies % NW == 0, "every wave copies whole kilobytes");
+  static constexpr int EPC = 16 / ES;  // elements per chunk
   unsigned voff[PER];
 
   // Chunk of this lane in copy j, as a k offset (KC).
@@ -143,29 +156,34 @@ struct TileCopy {
     }
   }
 
-  // base: the tile's first byte at this K step; end: the operand's bytes from
-  // there on; krem: K elements left at this step.
-  __device__ __forceinline__ void issue(char* lds, const char* base, int64_t end, int krem,
+  // base: the tile's first byte at this K step; end: the operand's bytes from there
+  // on (<= 0: the step does not exist, zeros arrive).
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(const char* base, int64_t end) {
+    const int records = end > 0x7fffffff ? 0x7fffffff : end < 0 ? 0 : (int)end;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, records, 0x00020000);
+  }
+  // Copy j; krem: K elements left at this step.
+  __device__ __forceinline__ void issue(int j, char* lds, __amdgpu_buffer_rsrc_t r, int krem,
                                         int wave, int lane) const {
-    const int records = end > 0x7fffffff ? 0x7fffffff : (int)end;
-    const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, records, 0x00020000);
-    const bool tail = !KS && krem < kStep;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (kCopies % NW != 0 && j * NW + wave >= kCopies) break;
-      unsigned v = voff[j];
-      if (tail && k_chunk(j, wave, lane) * EPC >= krem) v = kOutside;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          r, (__attribute__((address_space(3))) void*)(lds + (j * NW + wave) * 1024), 16, (int)v, 0,
-          0, 0);
-    }
+    unsigned v = voff[j];
+    if (!KS) v = k_chunk(j, wave, lane) * EPC < krem ? v : kOutside;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        r, (__attribute__((address_space(3))) void*)(lds + (j * NW + wave) * 1024), 16, (int)v, 0,
+        0, 0);
   }
 };
 
 // ---- reading a wave's fragments from LDS -----------------------------------
 __device__ __forceinline__ u32x4 lds_b128(const char* p) {
   return *(const __attribute__((address_space(3))) u32x4*)p;
+}
+
+// The transposing read: 16 lanes read 4 rows of 16 16-bit elements, 8 bytes each, and lane
+// i gets column i.  The restrict marks the access for the alias analysis, without
+// which the compiler waits for every copy in flight before each of these reads.
+__device__ __forceinline__ u32x2 lds_tr_b64(
+    __attribute__((address_space(3))) s16x4* __restrict__ p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
 }
 
 // S subtiles of 16 m (n) from subtile sub0 of a tile of ROWS.
@@ -178,7 +196,8 @@ struct Frag {
   __device__ __forceinline__ void init(int sub0, int lane) {
     const int r = lane & 15, q = lane >> 4;
     if constexpr (!KS) {
-      // M side: row 16 s + r.  N side: subtile t's row r = 4 q' + i is LDS row 16 q' + 4 t + i.
+      // M side: row 16 s + r.  N side, per 4 subtiles: subtile t's row r = 4 q' + i is
+      // LDS row 16 q' + 4 t + i.
       const int row = sub0 * 16 + (NSIDE ? (r >> 2) * 16 + (r & 3) : r);
       const int key = kc_key<NSIDE>(row);
       addr[0] = row * kStepBytes + (q ^ key) * 16;
@@ -200,13 +219,12 @@ struct Frag {
   // Fragment of subtile s, 64-byte half kk of the K step.
   __device__ __forceinline__ u32x4 get(char* tile, int s, int kk) const {
     if constexpr (!KS) {
-      return lds_b128(tile + addr[kk] + s * (NSIDE ? 4 : 16) * kStepBytes);
+      const int row = NSIDE ? (s >> 2) * 64 + (s & 3) * 4 : s * 16;
+      return lds_b128(tile + addr[kk] + row * kStepBytes);
     } else if constexpr (ES == 2) {
       typedef __attribute__((address_space(3))) s16x4* P;
       char* a = tile + addr[s] + kk * 32 * RB;
-      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)a));
-      const u32x2 hi =
-          __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(a + 4 * RB)));
+      const u32x2 lo = lds_tr_b64((P)a), hi = lds_tr_b64((P)(a + 4 * RB));
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
       const char* a = tile + addr[s] + kk * 16 * RB;
@@ -255,10 +273,12 @@ __device__ __forceinline__ void gate_grad(float da, float g, float u, float& dg,
 
 // Rows of the padded intermediate buffers are ldi elements apart; one row's
 // valid part is N elements.
-template <typename T, int EPI, int MT, bool BS>
+template <typename T, int EPI, bool BS>
 struct Epilogue {
   typedef typename Mma<T>::Acc Acc;
 
+  // acc[mt][t]: 16 m, and 64 n (gated: 32 of gate, 32 of up) in 4 subtiles.
+  template <int MT>
   static __device__ __forceinline__ void run(const GemmArgs& g, Acc (&acc)[MT][4], int prob,
                                              int slice, int m0, int n0, int lane) {
     const int r = lane & 15, q = lane >> 4;
@@ -393,18 +413,38 @@ struct Epilogue {
   }
 };
 
+// Waits until all but the wave's N newest copies have landed and its LDS reads are
+// done, then for the block's other waves.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
 // Bytes of a row up to the end of its last 16-byte chunk (rows are padded to whole chunks).
 __device__ __forceinline__ int64_t chunked(int64_t bytes) { return (bytes + 15) & ~(int64_t)15; }
 
 // ---- the kernel -------------------------------------------------------------
-template <typename T, int WM, int WN, int MT, bool AS, bool BS, int EPI>
-__global__ __launch_bounds__(WM* WN * 64) void k_dense(GemmArgs g) {
+// A block of WM x WN waves, each with MT x 4 G subtiles of 16 x 16.  Both halves' (64
+// bytes of K) fragments are held in registers: while one half is multiplied, the
+// other's are read.  The K step's only barrier lies between its halves: behind it the
+// next step's tiles are in LDS (their copies were issued one step earlier) and
+// nobody reads the present ones any more, which the copies of the step after next
+// then replace.  Each half is written as MT groups of NT products, with the LDS
+// reads and copies dealt to the groups and the groups kept in order, so that
+// the matrix cores, the LDS and the copies run side by side in one wave.
+//
+// 128 x 128 wave tiles (256 x 256, 4 waves) read 128 KB of fragments per K step
+// beside 64 KB of copies: at the LDS's 128 bytes a clock three quarters of the
+// products' 2048 clocks.  8 waves of 128 x 64 read 192 KB, which takes all of them.
+template <typename T, int WM, int WN, int MT, int G, bool AS, bool BS, int EPI>
+__global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
   constexpr bool GATED = EPI == kGated || EPI == kGatedMax || EPI == kPartGated;
-  constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * 64;
-  constexpr int ABYTES = BM * kStepBytes, BBYTES = BN * kStepBytes;
+  constexpr int NT = 4 * G;
+  constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
+  constexpr int ABYTES = BM * kStepBytes, BBYTES = BN * kStepBytes, BUF = ABYTES + BBYTES;
   constexpr int ES = sizeof(T), KB = kStepBytes / ES;
   typedef typename Mma<T>::Acc Acc;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * (ABYTES + BBYTES)];
+  __shared__ __attribute__((aligned(1024))) char smem[2 * BUF];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -419,61 +459,120 @@ __global__ __launch_bounds__(WM* WN * 64) void k_dense(GemmArgs g) {
   const int per = (total + g.slices - 1) / g.slices;
   const int s0 = id.slice * per, s1 = min(total, s0 + per);
 
-  TileCopy<T, BM, NW, AS, false, false> ca;
-  TileCopy<T, BN, NW, BS, true, GATED> cb;
+  typedef TileCopy<T, BM, NW, AS, false, false> CopyA;
+  typedef TileCopy<T, BN, NW, BS, true, GATED> CopyB;
+  CopyA ca;
+  CopyB cb;
   ca.init(wave, lane, g.lda, AS ? g.M - m0 : 0);
   cb.init(wave, lane, g.ldb, BS ? g.N - n0 : 0);
   Frag<T, BM, MT, AS, false> fa;
-  Frag<T, BN, 4, BS, true> fb;
+  Frag<T, BN, NT, BS, true> fb;
   fa.init(wm * MT, lane);
-  fb.init(wn * 4, lane);
+  fb.init(wn * NT, lane);
 
-  auto copy = [&](int step, char* lds) {
+  const char* const pa0 = g.a[id.prob];
+  const char* const pa1 = g.a[1];
+  const char* const pb0 = g.b[GATED ? (wave & 1) : 0];
+  const char* const pb1 = g.b[1];
+  // Where a step's tiles come from.
+  struct Source {
+    __amdgpu_buffer_rsrc_t a, b;
+    int krem;
+  };
+  auto source = [&](int step) {
     const int seg = step >= steps ? 1 : 0;
     const int k = (step - seg * steps) * KB;
-    {
-      const char* p = g.a[g.nprob > 1 ? id.prob : seg];
-      const int64_t off = AS ? k * g.lda + (int64_t)m0 * ES : m0 * g.lda + (int64_t)k * ES;
-      const int64_t all = AS ? (g.K - 1) * g.lda + chunked((int64_t)g.M * ES)
-                             : (g.M - 1) * g.lda + chunked((int64_t)g.K * ES);
-      ca.issue(lds, p + off, all - off, g.K - k, wave, lane);
-    }
-    {
-      const char* p = g.b[GATED ? (wave & 1) : seg];
-      const int64_t off = BS ? k * g.ldb + (int64_t)n0 * ES : n0 * g.ldb + (int64_t)k * ES;
-      const int64_t all = BS ? (g.K - 1) * g.ldb + chunked((int64_t)g.N * ES)
-                             : (g.N - 1) * g.ldb + chunked((int64_t)g.K * ES);
-      cb.issue(lds + ABYTES, p + off, all - off, g.K - k, wave, lane);
+    const bool live = step < s1;
+    const char* pa = seg ? pa1 : pa0;
+    const int64_t offa = AS ? k * g.lda + (int64_t)m0 * ES : m0 * g.lda + (int64_t)k * ES;
+    const int64_t alla = AS ? (g.K - 1) * g.lda + chunked((int64_t)g.M * ES)
+                            : (g.M - 1) * g.lda + chunked((int64_t)g.K * ES);
+    const char* pb = seg ? pb1 : pb0;
+    const int64_t offb = BS ? k * g.ldb + (int64_t)n0 * ES : n0 * g.ldb + (int64_t)k * ES;
+    const int64_t allb = BS ? (g.K - 1) * g.ldb + chunked((int64_t)g.N * ES)
+                            : (g.N - 1) * g.ldb + chunked((int64_t)g.K * ES);
+    return Source{CopyA::source(pa + offa, live ? alla - offa : 0),
+                  CopyB::source(pb + offb, live ? allb - offb : 0), g.K - k};
+  };
+  // Copies lo .. hi - 1 of a step's CopyA::PER + CopyB::PER.
+  auto copy = [&](const Source& s, char* lds, int lo, int hi) {
+#pragma unroll
+    for (int j = 0; j < CopyA::PER + CopyB::PER; ++j) {
+      if (j < lo || j >= hi) continue;
+      if (j < CopyA::PER)
+        ca.issue(j, lds, s.a, s.krem, wave, lane);
+      else
+        cb.issue(j - CopyA::PER, lds + ABYTES, s.b, s.krem, wave, lane);
     }
   };
+  constexpr int COPIES = CopyA::PER + CopyB::PER;
 
-  Acc acc[MT][4];
+  Acc acc[G * MT * 4];  // [group of 4 n subtiles][m subtile][n subtile]
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int t = 0; t < 4; ++t) acc[i][t] = Acc{};
+  for (int i = 0; i < G * MT * 4; ++i) acc[i] = Acc{};
 
-  if (s0 < s1) copy(s0, smem);
-  __syncthreads();
-  for (int s = s0; s < s1; ++s) {
-    char* cur = smem + ((s - s0) & 1) * (ABYTES + BBYTES);
-    if (s + 1 < s1) copy(s + 1, smem + ((s + 1 - s0) & 1) * (ABYTES + BBYTES));
+  u32x4 a0[MT], b0[NT], a1[MT], b1[NT];
+  // Fragments lo .. hi - 1, those of B first: every product needs them.
+  auto read = [&](u32x4(&a)[MT], u32x4(&b)[NT], char* tile, int kk, int lo, int hi) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      u32x4 b[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) b[t] = fb.get(cur + ABYTES, t, kk);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const u32x4 a = fa.get(cur, i, kk);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) acc[i][t] = Mma<T>::go(b[t], a, acc[i][t]);
-      }
+    for (int j = 0; j < MT + NT; ++j) {
+      if (j < lo || j >= hi) continue;
+      if (j < NT)
+        b[j] = fb.get(tile + ABYTES, j, kk);
+      else
+        a[j - NT] = fa.get(tile, j - NT, kk);
     }
-    __syncthreads();
+  };
+  auto multiply = [&](const u32x4& a, const u32x4(&b)[NT], int i) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) Mma<T>::go(b[t], a, acc[((t >> 2) * MT + i) * 4 + (t & 3)]);
+  };
+  // Reads per group: done two groups before the half's end, for their latency.
+  constexpr int RPG = (MT + NT + MT - 3) / (MT - 2);
+  constexpr int CPG = (COPIES + MT - 1) / MT;
+
+  {
+    const Source first = source(s0), second = source(s0 + 1);
+    copy(first, smem, 0, COPIES);
+    copy(second, smem + BUF, 0, COPIES);
   }
-  Epilogue<T, EPI, MT, BS>::run(g, acc, id.prob, id.slice, m0 + wm * MT * 16,
-                                n0 + wn * (GATED ? 32 : 64), lane);
+  wait_copies<COPIES>();
+  read(a0, b0, smem, 0, 0, MT + NT);
+  settle(acc);
+  char* cur = smem;
+  char* next = smem + BUF;
+  // An empty slice runs one step of zeros (no step of it is live): without a way
+  // around the loop the sums stay in their registers.
+  int s = s0;
+  do {
+    const Source after = source(s + 2);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      read(a1, b1, cur, 1, i * RPG, (i + 1) * RPG);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a0[i], b0, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_copies<0>();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      read(a0, b0, next, 0, i * RPG, (i + 1) * RPG);
+      copy(after, cur, i * CPG, (i + 1) * CPG);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a1[i], b1, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    char* t = cur;
+    cur = next;
+    next = t;
+  } while (++s < s1);
+  wait_copies<0>();
+  settle(acc);
+  Acc(&out)[G][MT][4] = reinterpret_cast<Acc(&)[G][MT][4]>(acc);
+#pragma unroll
+  for (int j = 0; j < G; ++j)
+    Epilogue<T, EPI, BS>::run(g, out[j], id.prob, id.slice, m0 + wm * MT * 16,
+                              n0 + (wn * G + j) * (GATED ? 32 : 64), lane);
 }
 
 // The epilogue of a product split over K: the slices' sums added in order, then as
@@ -531,25 +630,27 @@ __global__ __launch_bounds__(256) void k_dense_join(GemmArgs g) {
       for (int d = 1; d < 64; d *= 2) mx = max(mx, (unsigned)__shfl_xor((int)mx, d));
       if ((threadIdx.x & 63) == 0) atomicMax(g.row_max + m, mx);
     } else {
-      if (n < limit) Epilogue<T, EPI, 1, true>::tile(g, s, prob, 0, m, n);
+      if (n < limit) Epilogue<T, EPI, true>::tile(g, s, prob, 0, m, n);
     }
   }
 }
 
 // ---- launching --------------------------------------------------------------
-template <typename T, int WM, int WN, int MT, bool AS, bool BS, int EPI>
+template <typename T, int WM, int WN, int MT, int G, bool AS, bool BS, int EPI>
 hipError_t launch_tile(const GemmArgs& g, hipStream_t s) {
   const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.nprob * g.slices;
-  k_dense<T, WM, WN, MT, AS, BS, EPI><<<(unsigned)blocks, WM * WN * 64, 0, s>>>(g);
+  k_dense<T, WM, WN, MT, G, AS, BS, EPI><<<(unsigned)blocks, WM * WN * 64, 0, s>>>(g);
   return hipGetLastError();
 }
 
 template <typename T, bool AS, bool BS, int EPI>
 hipError_t launch_shape(const GemmArgs& g, int shape, hipStream_t s) {
   switch (shape) {
-    case kTile256: return launch_tile<T, 2, 4, 8, AS, BS, EPI>(g, s);
-    case kTile128: return launch_tile<T, 2, 2, 4, AS, BS, EPI>(g, s);
-    default: return launch_tile<T, 1, 4, 4, AS, BS, EPI>(g, s);
+    case kTile256:  // fp32 is bound by its products, not by the LDS: smaller wave tiles
+      if constexpr (sizeof(T) == 4) return launch_tile<T, 2, 4, 8, 1, AS, BS, EPI>(g, s);
+      return launch_tile<T, 2, 2, 8, 2, AS, BS, EPI>(g, s);
+    case kTile128: return launch_tile<T, 2, 2, 4, 1, AS, BS, EPI>(g, s);
+    default: return launch_tile<T, 1, 4, 4, 1, AS, BS, EPI>(g, s);
   }
 }
 
