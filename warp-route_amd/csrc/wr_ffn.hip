@@ -180,48 +180,74 @@ hipError_t launch_zero(void* p, int64_t bytes, hipStream_t s) {
 }
 
 // ---- the choice of tiles --------------------------------------------------------
-// A product's time is taken as rounds x (steps of a slice x time of a step + the
-// tile's fixed part) + what splitting costs; the shape and number of slices with the
-// least is chosen.
+// Tiles are dealt to the CUs in rounds.  Those of the last round, which fills the CUs
+// only in part, may be split over K into slices that fill it better and are
+// shorter; their sums go through memory and a second, short kernel.  The shape and
+// number of slices with the least estimated time are taken.
 struct ShapeCost {
   int bm, bn, per_cu;  // tile, blocks a CU holds
-  float step;          // us a K step of a tile takes with per_cu blocks on the CU
+  float step;          // us per 128 bytes of K, with per_cu blocks on the CU
+  float alone;         // the same with one
   float fixed;         // us per tile: first copies, epilogue
 };
-constexpr ShapeCost kCost[kShapes] = {
-    {256, 256, 1, 1.5f, 4.0f}, {128, 128, 2, 0.9f, 3.0f}, {64, 256, 2, 1.1f, 3.0f}};
+constexpr ShapeCost kCost16[kShapes] = {{256, 256, 1, 1.48f, 1.48f, 5.0f},
+                                        {128, 128, 2, 0.95f, 0.60f, 4.0f},
+                                        {64, 256, 2, 0.95f, 0.60f, 4.0f}};
+constexpr ShapeCost kCost32[kShapes] = {{256, 256, 1, 7.7f, 7.7f, 6.0f},
+                                        {128, 128, 2, 4.0f, 2.4f, 4.0f},
+                                        {64, 256, 2, 4.0f, 2.4f, 4.0f}};
 constexpr int kCUs = 256;
 constexpr int kMaxSlices = 32;
-constexpr int64_t kMaxPartBytes = (int64_t)256 << 20;
+constexpr int64_t kMaxPartBytes = (int64_t)512 << 20;
 
 struct Plan {
-  int shape, slices, tiles_m, tiles_n;
-  int64_t ldp;
+  int shape, slices, tiles_m, tiles_n, tiles, whole;
   size_t part_bytes;
 };
 
-// M x N x K per problem; gated: N columns of each of two matrices.
-Plan plan_of(int M, int N, int K, int es, int nseg, int nprob, bool gated) {
+float rounds_us(const ShapeCost& c, int64_t blocks, int steps) {
+  const int64_t cap = (int64_t)kCUs * c.per_cu, rest = blocks % cap;
+  const float full = steps * c.step + c.fixed;
+  return blocks / cap * full +
+         (rest == 0 ? 0.0f : rest <= kCUs ? steps * c.alone + c.fixed : full);
+}
+
+// Rows of m up to which a product of two K-contiguous operands goes to k_dense_rows.
+constexpr int kRowsMax = 16;
+// 32 rows of B a block where that leaves 2 blocks a CU, else 16; 8 waves a block
+// where there are fewer blocks than CUs, else 4.
+Plan plan_rows(int N, int K, int es, bool gated, bool any) {
+  const int64_t steps = ((int64_t)K * es + 127) / 128;
+  const bool wide = !any && (N + (gated ? 15 : 31)) / (gated ? 16 : 32) >= 2 * kCUs;
+  const int rows = (wide ? 32 : 16) / (gated ? 2 : 1), blocks = (N + rows - 1) / rows;
+  const int waves = blocks < kCUs && steps >= 16 ? 8 : 4;
+  return {any ? kRowsAny : wide ? kRows32 : kRows16, waves, 1, blocks, blocks, blocks, 0};
+}
+
+// M x N x K per problem; gated: N columns of each of two matrices; rows: the few-row
+// kernels, any: for rows of any length.
+Plan plan_of(int M, int N, int K, int es, int nseg, int nprob, bool gated, bool rows, bool any) {
   const int kb = 128 / es;
   const int steps = (K + kb - 1) / kb * nseg;
-  const float rate = es == 4 ? 8.0f : 1.0f;  // fp32 steps: 16 times the time of half the K
+  if (rows) return plan_rows(N, K, es, gated, any);
   Plan best{};
   float best_us = 0;
-  const int64_t ldp = round_up(N, 64);
   for (int shape = 0; shape < kShapes; ++shape) {
-    const ShapeCost& c = kCost[shape];
+    const ShapeCost& c = es == 4 ? kCost32[shape] : kCost16[shape];
     const int64_t tm = (M + c.bm - 1) / c.bm, bn = gated ? c.bn / 2 : c.bn;
-    const int64_t tn = (N + bn - 1) / bn;
-    for (int S = 1; S <= kMaxSlices; S *= 2) {
-      const size_t part = S == 1 ? 0 : (size_t)S * nprob * M * ldp * 4 * (gated ? 2 : 1);
-      if (S > 1 && (steps / S < 4 || part > (size_t)kMaxPartBytes)) break;
-      const int64_t blocks = tm * tn * nprob * S;
-      const int64_t rounds = (blocks + (int64_t)kCUs * c.per_cu - 1) / ((int64_t)kCUs * c.per_cu);
-      const int per = (steps + S - 1) / S;
-      const float us = rounds * (per * c.step * rate + c.fixed) +
-                       (S == 1 ? 0.0f : 4.0f + (float)part * 2 / 4e6f);
-      if (best.tiles_m == 0 || us < best_us) {
-        best = {shape, S, (int)tm, (int)tn, ldp, part};
+    const int64_t tn = (N + bn - 1) / bn, tiles = tm * tn * nprob;
+    const int64_t cap = (int64_t)kCUs * c.per_cu, rest = tiles % cap;
+    for (int S = 1; S <= kMaxSlices && S * 2 <= std::max(2, steps); ++S) {
+      const int64_t whole = S == 1 ? tiles : tiles - rest;
+      const int64_t part = (tiles - whole) * S * c.bm * c.bn * 4;
+      if (S > 1 && (rest == 0 || part > kMaxPartBytes)) break;
+      // Sums of rows past M are neither written nor read.
+      const float moved = 2.0f * part * std::min(1.0f, (float)M / (tm * c.bm));
+      const float us = rounds_us(c, whole, steps) +
+                       (S == 1 ? 0.0f
+                               : rounds_us(c, rest * S, (steps + S - 1) / S) + 4.0f + moved / 4e6f);
+      if (best.tiles == 0 || us < best_us) {
+        best = {shape, S, (int)tm, (int)tn, (int)tiles, (int)whole, (size_t)part};
         best_us = us;
       }
     }
@@ -251,14 +277,15 @@ struct Call {
   }
   bool go() const { return !dry() && err == hipSuccess; }
 
-  // An operand matrix with whole 16-byte rows: itself, or a padded copy.
+  // An operand matrix with whole 16-byte rows: itself, or a padded copy.  any_row: the
+  // product takes rows of any length.
   struct Mat {
     const char* p;
     int64_t ld;  // bytes
   };
-  Mat rows16(const void* p, int64_t rows, int cols) {
+  Mat rows16(const void* p, int64_t rows, int cols, bool any_row = false) {
     const int64_t bytes = (int64_t)cols * es(), ld = round_up(bytes, 16);
-    if (ld == bytes) return {(const char*)p, ld};
+    if (any_row || ld == bytes) return {(const char*)p, bytes};
     char* c = take(rows * ld);
     if (go()) check(launch_pad(p, c, rows, cols, ld, es(), stream));
     return {c, ld};
@@ -270,13 +297,17 @@ struct Call {
   void product(GemmArgs g, int form) {
     const bool gated = form == kFormGated || form == kFormGatedMax;
     if (g.M == 0 || g.N == 0) return;
-    const Plan pl = plan_of(g.M, g.N, g.K, es(), g.nseg, g.nprob, gated);
+    const bool rows = g.M <= kRowsMax && form != kFormGateGrad && form != kFormKcKs &&
+                      form != kFormKsKs;
+    const bool any = g.lda % 16 != 0 || g.ldb % 16 != 0;
+    const Plan pl = plan_of(g.M, g.N, g.K, es(), g.nseg, g.nprob, gated, rows, any);
     reserve_part(pl);
     if (!go()) return;
     g.slices = pl.slices;
     g.tiles_m = pl.tiles_m;
     g.tiles_n = pl.tiles_n;
-    g.ldp = pl.ldp;
+    g.tiles = pl.tiles;
+    g.whole = pl.whole;
     g.part = ws + part_at;
     const int oes = int8 ? elem_bytes(g.out_dtype) : es();
     g.vec = g.ldo * oes % 16 == 0;
@@ -296,7 +327,7 @@ GemmArgs gemm(const Call::Mat& a, const Call::Mat& b, int M, int N, int K) {
   g.M = M;
   g.N = N;
   g.K = K;
-  g.nseg = g.nprob = g.slices = 1;
+  g.nseg = g.nprob = 1;
   return g;
 }
 
@@ -304,9 +335,10 @@ void run_forward(Call& c, const wr_ffn_args& a) {
   const int T = a.batch_size, h = a.hidden_dim, I = a.intermediate_dim;
   const int64_t Ip = round_up(I, 64);
   const bool keep = a.saved_act != nullptr;
-  const Call::Mat x = c.rows16(a.x, T, h);
-  const Call::Mat wg = c.rows16(a.w_gate, I, h), wu = c.rows16(a.w_up, I, h);
-  const Call::Mat wd = c.rows16(a.w_down, h, I);
+  const bool few = T <= kRowsMax;
+  const Call::Mat x = c.rows16(a.x, T, h, few);
+  const Call::Mat wg = c.rows16(a.w_gate, I, h, few), wu = c.rows16(a.w_up, I, h, few);
+  const Call::Mat wd = c.rows16(a.w_down, h, I, few);
   char* own = c.take((int64_t)T * Ip * c.es());  // sized whether saved or not
   const Call::Mat act{keep ? (const char*)a.saved_act : own, Ip * c.es()};
 
@@ -371,8 +403,9 @@ void run_backward(Call& c, const wr_ffn_args& a, bool dx, bool dwg, bool dwu, bo
 }
 
 void run_int8(Call& c, const wr_int8_args& a) {
-  const Call::Mat x = c.rows16(a.x, a.rows, a.in_features);
-  const Call::Mat w = c.rows16(a.w, a.out_features, a.in_features);
+  const bool few = a.rows <= kRowsMax;
+  const Call::Mat x = c.rows16(a.x, a.rows, a.in_features, few);
+  const Call::Mat w = c.rows16(a.w, a.out_features, a.in_features, few);
   GemmArgs g = gemm(x, w, a.rows, a.out_features, a.in_features);
   g.out[0] = a.out;
   g.ldo = a.out_features;
@@ -391,8 +424,9 @@ void run_ffn_int8(Call& c, const wr_ffn_int8_args& a) {
   float* act = (float*)c.take(T * Ip * 4);
   int8_t* aq = (int8_t*)c.take(T * Ip);
   float* sa = (float*)c.take((int64_t)T * 4);
-  const Call::Mat wg = c.rows16(a.w_gate, I, h), wu = c.rows16(a.w_up, I, h);
-  const Call::Mat wd = c.rows16(a.w_down, h, I);
+  const bool few = T <= kRowsMax;
+  const Call::Mat wg = c.rows16(a.w_gate, I, h, few), wu = c.rows16(a.w_up, I, h, few);
+  const Call::Mat wd = c.rows16(a.w_down, h, I, few);
   if (c.go())
     c.check(launch_quantize<false>(a.x, a.dtype, h, T, h, nullptr, xq, hp, sx, amax, c.stream));
   GemmArgs g = gemm({(const char*)xq, hp}, wg, T, I, h);

@@ -15,8 +15,8 @@
 //
 // Tiles.  A K step is 128 bytes of K: 64 16-bit elements, 128 int8, 32 fp32.
 // Both operand tiles of a step are copied from memory straight into LDS
-// (buffer_load ... lds, 16 bytes a lane), into one of two buffers while the
-// other is multiplied.  The copy's buffer descriptor ends at the operand's
+// (buffer_load ... lds, 16 bytes a lane), into a ring of 2 or 4 buffers of which
+// one is multiplied.  The copy's buffer descriptor ends at the operand's
 // last element, so rows past the end arrive as zeros without a branch; K
 // tails and column tails give their lanes an offset behind the descriptor.
 //
@@ -57,7 +57,7 @@ constexpr unsigned kOutside = 0x80000000u;  // offset behind every descriptor
 // The 16-bit and int8 instructions are written as assembly with the sums tied to
 // accumulation registers: the compiler's own register allocation moves the sums of
 // a 128 x 128 wave tile (all 256 accumulation registers) between registers in the
-// loop.  The waits its hazard pass would add are held by construction: fragments
+// loop (add is the compiler's form, for few sums).  The waits its hazard pass would add are held by construction: fragments
 // come from LDS reads alone (no vector instruction writes them), equal sums are at
 // least NT products apart, and settle() stands between the sums' first and last
 // use and any other instruction on them.
@@ -69,12 +69,20 @@ struct Mma<bf16> {
   static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
+  static __device__ __forceinline__ Acc add(u32x4 a, u32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
 };
 template <>
 struct Mma<f16> {
   typedef f32x4 Acc;
   static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  }
+  static __device__ __forceinline__ Acc add(u32x4 a, u32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
 template <>
@@ -83,17 +91,23 @@ struct Mma<int8_t> {
   static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
     asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
+  static __device__ __forceinline__ Acc add(u32x4 a, u32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a),
+                                                 __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+  }
 };
 // fp32: lane group q holds k = 4 q .. 4 q + 3, one element per MFMA.
 template <>
 struct Mma<float> {
   typedef f32x4 Acc;
-  static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
+  static __device__ __forceinline__ Acc add(u32x4 a, u32x4 b, Acc c) {
     const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+    return c;
   }
+  static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) { c = add(a, b, c); }
 };
 
 // Orders all accumulators' values between the assembly products and other instructions,
@@ -277,58 +291,44 @@ template <typename T, int EPI, bool BS>
 struct Epilogue {
   typedef typename Mma<T>::Acc Acc;
 
-  // acc[mt][t]: 16 m, and 64 n (gated: 32 of gate, 32 of up) in 4 subtiles.
-  template <int MT>
-  static __device__ __forceinline__ void run(const GemmArgs& g, Acc (&acc)[MT][4], int prob,
-                                             int slice, int m0, int n0, int lane) {
-    const int r = lane & 15, q = lane >> 4;
+  // 16 m from m0, and 64 n from n0 (gated: 32 of gate, 32 of up) in 4 subtiles.
+  static __device__ __forceinline__ void run(const GemmArgs& g, const Acc (&acc)[4], int prob,
+                                             int m0, int n0, int lane) {
+    const int q = lane >> 4, m = m0 + (lane & 15);
+    if constexpr (EPI == kGatedMax) {
+      gated_max(g, acc, m, n0 + q * 8);
+    } else if (m >= g.M) {
+      return;
+    } else if constexpr (EPI == kGated) {
+      float gg[8], uu[8];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int m = m0 + mt * 16 + r;
-      if (EPI == kGatedMax) {
-        gated_max(g, acc[mt], m, n0, q);
-        continue;
+      for (int i = 0; i < 8; ++i) {
+        gg[i] = acc[i / 4][i % 4];
+        uu[i] = acc[i / 4 + 2][i % 4];
       }
-      if (m >= g.M) continue;
-      if constexpr (EPI == kGated) {
-        gated(g, acc[mt], m, n0 + q * 8);
-      } else if constexpr (EPI == kPartGated) {
-        const int64_t at = ((int64_t)slice * g.M + m) * 2 * g.ldp;
-        const int n = n0 + q * 8;
+      gated<8>(g, gg, uu, m, n0 + q * 8);
+    } else if constexpr (EPI == kStore && !BS) {
+      float v[16];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          if (n + (t & 1) * 4 < g.N)
-            *(Acc*)(reinterpret_cast<char*>(g.part) +
-                    (at + (t >> 1) * g.ldp + n + (t & 1) * 4) * 4) = acc[mt][t];
-      } else if constexpr (EPI == kStore && !BS) {
-        float v[16];
+      for (int i = 0; i < 16; ++i) v[i] = acc[i / 4][i % 4];
+      const int n = n0 + q * 16;
+      T* p = (T*)g.out[prob] + (int64_t)m * g.ldo + n;
+      constexpr int V = 16 / sizeof(T);
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+      for (int i = 0; i < 16; i += V) store_run<T, V>(p + i, v + i, g.N - n - i, g.vec);
+    } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[t * 4 + i] = acc[mt][t][i];
-        const int n = n0 + q * 16;
-        T* p = (T*)g.out[prob] + (int64_t)m * g.ldo + n;
-        constexpr int V = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < 16; i += V) store_run<T, V>(p + i, v + i, g.N - n - i, g.vec);
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int n = n0 + (BS ? t * 16 + q * 4 : q * 16 + t * 4);
-          // dg and du rows are read in whole 16-byte chunks: their zeros past N too.
-          if (n < (EPI == kGateGrad ? (g.N + 7) & ~7 : g.N)) tile(g, acc[mt][t], prob, slice, m, n);
-        }
+      for (int t = 0; t < 4; ++t) {
+        const int n = n0 + (BS ? t * 16 + q * 4 : q * 16 + t * 4);
+        // dg and du rows are read in whole 16-byte chunks: their zeros past N too.
+        if (n < (EPI == kGateGrad ? (g.N + 7) & ~7 : g.N)) tile(g, acc[t], prob, m, n);
       }
     }
   }
 
   // Four consecutive n of one m.
-  static __device__ __forceinline__ void tile(const GemmArgs& g, Acc a, int prob, int slice, int m,
-                                              int n) {
-    if constexpr (EPI == kPart) {
-      const int64_t at = (((int64_t)slice * g.nprob + prob) * g.M + m) * g.ldp + n;
-      *(Acc*)(reinterpret_cast<char*>(g.part) + at * 4) = a;  // ldp covers the tail
-    } else if constexpr (EPI == kStore) {
+  static __device__ __forceinline__ void tile(const GemmArgs& g, Acc a, int prob, int m, int n) {
+    if constexpr (EPI == kStore) {
       const float v[4] = {a[0], a[1], a[2], a[3]};
       store_run<T, 4>((T*)g.out[prob] + (int64_t)m * g.ldo + n, v, g.N - n, g.vec);
     } else if constexpr (EPI == kGateGrad) {
@@ -356,60 +356,59 @@ struct Epilogue {
     }
   }
 
-  // 8 gate and 8 up sums of the same n (acc[0..1] and acc[2..3]).  The buffers'
-  // rows are padded to ldi (a multiple of 64), so whole vectors are stored.
-  static __device__ __forceinline__ void gated(const GemmArgs& g, const Acc (&acc)[4], int m,
-                                               int n) {
-    if (n >= g.N) return;
-    float a[8], gg[8], uu[8];
+  // C gate and up sums of the same n.  The buffers' rows are padded to ldi (a multiple of
+  // 64) and the sums past N are zero, so whole vectors are stored.
+  template <int C>
+  static __device__ __forceinline__ void gated(const GemmArgs& g, const float (&gg)[C],
+                                               const float (&uu)[C], int m, int n) {
+    if (n >= ((g.N + 7) & ~7)) return;
+    float a[C];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        gg[t * 4 + i] = acc[t][i];
-        uu[t * 4 + i] = acc[t + 2][i];
-        a[t * 4 + i] = silu(acc[t][i]) * acc[t + 2][i];
-      }
+    for (int i = 0; i < C; ++i) a[i] = silu(gg[i]) * uu[i];
     const int64_t at = (int64_t)m * g.ldi + n;
-    constexpr int V = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;
+    constexpr int V = 16 / sizeof(T) < C ? 16 / sizeof(T) : C;
 #pragma unroll
-    for (int i = 0; i < 8; i += V) store_run<T, V>((T*)g.out[0] + at + i, a + i, V, true);
+    for (int i = 0; i < C; i += V) store_run<T, V>((T*)g.out[0] + at + i, a + i, V, true);
     if (g.out[1] != nullptr) {
 #pragma unroll
-      for (int i = 0; i < 8; i += 4) {
+      for (int i = 0; i < C; i += 4) {
         store_run<float, 4>((float*)g.out[1] + at + i, gg + i, 4, true);
         store_run<float, 4>((float*)g.out[2] + at + i, uu + i, 4, true);
       }
     }
   }
 
-  // int8: a = silu(g) u in fp32 with its row maxima of |a| (as fp32 bits: the
+  // int8: a = silu(g) u in fp32 of 8 n from n, with the row maxima of |a| (as fp32 bits: the
   // maximum of non-negative floats is that of their bits, in any order).
   static __device__ __forceinline__ void gated_max(const GemmArgs& g, const Acc (&acc)[4], int m,
-                                                   int n0, int q) {
-    const int n = n0 + q * 8;
+                                                   int n) {
     unsigned mx = 0;
-    if (m < g.M && n < g.N) {
-      const float sm = g.row_scale[m];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = n + t * 4 + i;
-          v[i] = 0.0f;
-          if (c < g.N) {
-            const float gg = (float)acc[t][i] * sm * g.col_scale[0][c];
-            v[i] = silu(gg) * ((float)acc[t + 2][i] * sm * g.col_scale[1][c]);
-          }
-          mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
-        }
-        store_run<float, 4>((float*)g.out[0] + (int64_t)m * g.ldi + n + t * 4, v, 4, true);
-      }
+    if (m < g.M) {
+      mx = scaled_gate(g, acc[0], acc[2], m, n);
+      mx = max(mx, scaled_gate(g, acc[1], acc[3], m, n + 4));
     }
     mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
     mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
-    if (q == 0 && m < g.M) atomicMax(g.row_max + m, mx);
+    if ((threadIdx.x & 63) < 16 && m < g.M) atomicMax(g.row_max + m, mx);
+  }
+  // Four n; returns their maximum.
+  static __device__ __forceinline__ unsigned scaled_gate(const GemmArgs& g, Acc gate, Acc up, int m,
+                                                         int n) {
+    unsigned mx = 0;
+    if (n >= g.N) return mx;
+    const float sm = g.row_scale[m];
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = 0.0f;
+      if (n + i < g.N) {
+        const float gg = (float)gate[i] * sm * g.col_scale[0][n + i];
+        v[i] = silu(gg) * ((float)up[i] * sm * g.col_scale[1][n + i]);
+      }
+      mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
+    }
+    store_run<float, 4>((float*)g.out[0] + (int64_t)m * g.ldi + n, v, 4, true);
+    return mx;
   }
 };
 
@@ -427,8 +426,8 @@ __device__ __forceinline__ int64_t chunked(int64_t bytes) { return (bytes + 15) 
 // A block of WM x WN waves, each with MT x 4 G subtiles of 16 x 16.  Both halves' (64
 // bytes of K) fragments are held in registers: while one half is multiplied, the
 // other's are read.  The K step's only barrier lies between its halves: behind it the
-// next step's tiles are in LDS (their copies were issued one step earlier) and
-// nobody reads the present ones any more, which the copies of the step after next
+// next step's tiles are in LDS (their copies were issued SLOTS - 1 steps earlier)
+// and nobody reads the present ones any more, which the copies of step s + SLOTS
 // then replace.  Each half is written as MT groups of NT products, with the LDS
 // reads and copies dealt to the groups and the groups kept in order, so that
 // the matrix cores, the LDS and the copies run side by side in one wave.
@@ -436,27 +435,25 @@ __device__ __forceinline__ int64_t chunked(int64_t bytes) { return (bytes + 15) 
 // 128 x 128 wave tiles (256 x 256, 4 waves) read 128 KB of fragments per K step
 // beside 64 KB of copies: at the LDS's 128 bytes a clock three quarters of the
 // products' 2048 clocks.  8 waves of 128 x 64 read 192 KB, which takes all of them.
-template <typename T, int WM, int WN, int MT, int G, bool AS, bool BS, int EPI>
+template <typename T, int WM, int WN, int MT, int G, int SLOTS, bool AS, bool BS, int EPI>
 __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
-  constexpr bool GATED = EPI == kGated || EPI == kGatedMax || EPI == kPartGated;
+  constexpr bool GATED = EPI == kGated || EPI == kGatedMax;
   constexpr int NT = 4 * G;
   constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
   constexpr int ABYTES = BM * kStepBytes, BBYTES = BN * kStepBytes, BUF = ABYTES + BBYTES;
   constexpr int ES = sizeof(T), KB = kStepBytes / ES;
   typedef typename Mma<T>::Acc Acc;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * BUF];
+  __shared__ __attribute__((aligned(1024))) char smem[SLOTS * BUF];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
-  // Block -> (slice, problem, tile).  Consecutive blocks go to the 8 XCDs in
-  // turn, so each XCD takes one run of the tile order; within it 8 m tiles
-  // advance together along n, for both operands' reuse in the XCD's L2.
-  const TileId id = tile_of(g, (int)blockIdx.x, (int)gridDim.x);
+  const TileId id = tile_of(g, (int)blockIdx.x);
   const int m0 = id.m * BM, n0 = id.n * (GATED ? BN / 2 : BN);
   const int steps = (g.K + KB - 1) / KB, total = steps * g.nseg;
-  const int per = (total + g.slices - 1) / g.slices;
+  const int slices = id.tail < 0 ? 1 : g.slices;
+  const int per = (total + slices - 1) / slices;
   const int s0 = id.slice * per, s1 = min(total, s0 + per);
 
   typedef TileCopy<T, BM, NW, AS, false, false> CopyA;
@@ -531,21 +528,20 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
   constexpr int RPG = (MT + NT + MT - 3) / (MT - 2);
   constexpr int CPG = (COPIES + MT - 1) / MT;
 
-  {
-    const Source first = source(s0), second = source(s0 + 1);
-    copy(first, smem, 0, COPIES);
-    copy(second, smem + BUF, 0, COPIES);
-  }
-  wait_copies<COPIES>();
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) copy(source(s0 + i), smem + i * BUF, 0, COPIES);
+  wait_copies<(SLOTS - 1) * COPIES>();
   read(a0, b0, smem, 0, 0, MT + NT);
   settle(acc);
-  char* cur = smem;
-  char* next = smem + BUF;
+  int at = 0;
   // An empty slice runs one step of zeros (no step of it is live): without a way
   // around the loop the sums stay in their registers.
   int s = s0;
   do {
-    const Source after = source(s + 2);
+    const Source after = source(s + SLOTS);
+    char* const cur = smem + at * BUF;
+    at = at + 1 == SLOTS ? 0 : at + 1;
+    char* const next = smem + at * BUF;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       read(a1, b1, cur, 1, i * RPG, (i + 1) * RPG);
@@ -553,7 +549,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
       multiply(a0[i], b0, i);
       __builtin_amdgcn_sched_barrier(0);
     }
-    wait_copies<0>();
+    wait_copies<(SLOTS - 2) * COPIES>();
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       read(a0, b0, next, 0, i * RPG, (i + 1) * RPG);
@@ -562,119 +558,301 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
       multiply(a1[i], b1, i);
       __builtin_amdgcn_sched_barrier(0);
     }
-    char* t = cur;
-    cur = next;
-    next = t;
   } while (++s < s1);
   wait_copies<0>();
   settle(acc);
-  Acc(&out)[G][MT][4] = reinterpret_cast<Acc(&)[G][MT][4]>(acc);
+  // A slice stores its sums as they lie in the registers.
+  Acc* const part = id.tail < 0 ? nullptr
+                                : (Acc*)g.part + ((int64_t)(id.tail * g.slices + id.slice) * NW + wave) *
+                                                     (G * MT * 4 * 64) + lane;
 #pragma unroll
   for (int j = 0; j < G; ++j)
-    Epilogue<T, EPI, BS>::run(g, out[j], id.prob, id.slice, m0 + wm * MT * 16,
-                              n0 + (wn * G + j) * (GATED ? 32 : 64), lane);
-}
-
-// The epilogue of a product split over K: the slices' sums added in order, then as
-// in k_dense.  One thread per 4 columns; blockIdx.y counts rows (and problems).
-template <typename T, int EPI>
-__global__ __launch_bounds__(256) void k_dense_join(GemmArgs g) {
-  typedef typename Mma<T>::Acc Acc;
-  constexpr bool GATED = EPI == kGated || EPI == kGatedMax;
-  const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
-  const int limit = EPI == kStore || EPI == kScale ? g.N : (g.N + 7) & ~7;
-  for (int64_t row = blockIdx.y; row < (int64_t)g.M * g.nprob; row += gridDim.y) {
-    const int prob = (int)(row / g.M), m = (int)(row % g.M);
-    const int64_t ld = GATED ? 2 * g.ldp : g.ldp;
-    const Acc* p = (const Acc*)g.part + (row * ld + n) / 4;
-    const int64_t step = (int64_t)g.nprob * g.M * ld / 4;
-    Acc s = Acc{}, u = Acc{};
-    if (n < g.N) {
-      for (int i = 0; i < g.slices; ++i) {
-        s += p[i * step];
-        if (GATED) u += p[i * step + g.ldp / 4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const Acc(&piece)[4] = *reinterpret_cast<Acc(*)[4]>(&acc[(j * MT + i) * 4]);
+      const int m = m0 + (wm * MT + i) * 16;
+      if (part == nullptr) {
+        Epilogue<T, EPI, BS>::run(g, piece, id.prob, m, n0 + (wn * G + j) * (GATED ? 32 : 64), lane);
+      } else if (m < g.M) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) part[((j * MT + i) * 4 + t) * 64] = piece[t];
       }
     }
+}
+
+// The tiles split over K: their slices' sums added in order, then as in k_dense.  One
+// wave per 16 m x 64 n (gated: 32 of each matrix) of a tile.
+template <typename T, int WM, int WN, int MT, int G, bool BS, int EPI>
+__global__ __launch_bounds__(256) void k_dense_join(GemmArgs g) {
+  constexpr bool GATED = EPI == kGated || EPI == kGatedMax;
+  constexpr int NW = WM * WN, PIECES = NW * G * MT;
+  typedef typename Mma<T>::Acc Acc;
+  const int lane = threadIdx.x & 63;
+  const int64_t piece = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int tail = (int)(piece / PIECES), rest = (int)(piece % PIECES);
+  const int wave = rest / (G * MT), j = rest / MT % G, i = rest % MT;
+  if (tail >= g.tiles - g.whole) return;
+  const TileId id = tile_at(g, g.whole + tail);
+  const int m0 = id.m * (WM * MT * 16) + (wave / WN * MT + i) * 16;
+  if (m0 >= g.M) return;
+  const int n0 = (id.n * WN * G + wave % WN * G + j) * (GATED ? 32 : 64);
+  const Acc* p = (const Acc*)g.part + ((int64_t)tail * g.slices * NW + wave) * (G * MT * 4 * 64) +
+                 (j * MT + i) * 4 * 64 + lane;
+  Acc acc[4] = {};
+  for (int s = 0; s < g.slices; ++s)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[t] += p[(int64_t)s * NW * (G * MT * 4 * 64) + t * 64];
+  Epilogue<T, EPI, BS>::run(g, acc, id.prob, m0, n0, lane);
+}
+
+// ---- few rows of m ---------------------------------------------------------
+// M <= 16: bound by the bytes of B, which are read once.  A block owns 16 S rows of B
+// (gated: half of them of gate, the same n of up) and splits K over its waves,
+// whose sums meet in LDS: one launch, no sums through memory.
+//
+// k_dense_rows: each wave copies its part of K into a ring of its own in LDS, 128 bytes of
+// 8 rows per copy, with kRowSlots - 1 steps in flight and no barrier.
+// 16 tokens, gate and up of 4096 x 14336 fp16 (235 MB): 44 us, 5.3 TB/s; loads straight
+// into the products' registers (16 rows x 64 bytes per load) take 61 us.  2, 3, 4 and
+// 6 slots with 2 to 8 waves: 3 slots and 4 waves are within 3% of the best of them
+// for every product measured.
+constexpr int kRowSlots = 3;
+
+// Joins the waves' sums (acc[S] of each) in LDS and runs the epilogue.
+template <typename T, int S, int EPI>
+__device__ __forceinline__ void join_waves(const GemmArgs& g, typename Mma<T>::Acc (&acc)[S],
+                                           char* lds, int n0, int wave, int waves, int lane) {
+  constexpr bool GATED = EPI == kGated || EPI == kGatedMax;
+  typedef typename Mma<T>::Acc Acc;
+  const int r = lane & 15, q = lane >> 4;
+  Acc* const sums = (Acc*)lds;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < S; ++i) sums[(wave * S + i) * 64 + lane] = acc[i];
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+    for (int w = 1; w < waves; ++w) acc[i] += sums[(w * S + i) * 64 + lane];
+  const int m = r;
+  if constexpr (!GATED) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const int n = n0 + i * 16 + q * 4;
+      if (m < g.M && n < g.N) Epilogue<T, EPI, true>::tile(g, acc[i], 0, m, n);
+    }
+  } else {
+    Acc up = acc[S - 1];
+    if (S == 1) {  // lane groups 0 and 1 hold gate, 2 and 3 the same n of up
+      i32x4 bits = __builtin_bit_cast(i32x4, up);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bits[i] = __shfl_xor((int)bits[i], 32);
+      up = __builtin_bit_cast(Acc, bits);
+    }
+    const int n = n0 + q * 4;
+    const bool mine = m < g.M && (S == 2 || q < 2);
     if constexpr (EPI == kGated) {
-      if (n >= limit) continue;
-      float a[4], gg[4], uu[4];
+      if (!mine) return;
+      float gg[4], uu[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        gg[i] = s[i];
-        uu[i] = u[i];
-        a[i] = silu(s[i]) * u[i];
+        gg[i] = n + i < g.N ? acc[0][i] : 0.0f;
+        uu[i] = n + i < g.N ? up[i] : 0.0f;
       }
-      const int64_t at = (int64_t)m * g.ldi + n;
-      store_run<T, 4>((T*)g.out[0] + at, a, 4, true);
-      if (g.out[1] != nullptr) {
-        store_run<float, 4>((float*)g.out[1] + at, gg, 4, true);
-        store_run<float, 4>((float*)g.out[2] + at, uu, 4, true);
-      }
-    } else if constexpr (EPI == kGatedMax) {
-      unsigned mx = 0;
-      if (n < limit) {
-        float v[4];
-        const float sm = g.row_scale[m];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = 0.0f;
-          if (n + i < g.N) {
-            const float gg = (float)s[i] * sm * g.col_scale[0][n + i];
-            v[i] = silu(gg) * ((float)u[i] * sm * g.col_scale[1][n + i]);
-          }
-          mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
-        }
-        store_run<float, 4>((float*)g.out[0] + (int64_t)m * g.ldi + n, v, 4, true);
-      }
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) mx = max(mx, (unsigned)__shfl_xor((int)mx, d));
-      if ((threadIdx.x & 63) == 0) atomicMax(g.row_max + m, mx);
+      Epilogue<T, EPI, true>::template gated<4>(g, gg, uu, m, n);
     } else {
-      if (n < limit) Epilogue<T, EPI, true>::tile(g, s, prob, 0, m, n);
+      unsigned mx = mine ? Epilogue<T, EPI, true>::scaled_gate(g, acc[0], up, m, n) : 0;
+      mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
+      mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
+      if (q == 0 && m < g.M) atomicMax(g.row_max + m, mx);
     }
   }
 }
 
+template <typename T, int S, int EPI>
+__global__ __launch_bounds__(512) void k_dense_rows(GemmArgs g) {
+  constexpr bool GATED = EPI == kGated || EPI == kGatedMax;
+  constexpr int ES = sizeof(T), KB = kStepBytes / ES, EPC = 16 / ES;
+  constexpr int COPIES = 2 * S + 2, SLOT = COPIES * 1024;  // 16 S rows of B, 16 of A
+  typedef typename Mma<T>::Acc Acc;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [wave][kRowSlots][SLOT]
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int n0 = blockIdx.x * (GATED ? 8 * S : 16 * S);
+  char* const ring = smem + wave * (kRowSlots * SLOT);
+
+  // Copy j: rows 8 j .. 8 j + 7 of B's tile, then of A.
+  auto copy = [&](int step, char* slot, bool live) {
+    const int k = step * KB;
+#pragma unroll
+    for (int j = 0; j < COPIES; ++j) {
+      const int lr = (j < 2 * S ? j : j - 2 * S) * 8 + (lane >> 3);  // row in the tile
+      const int chunk = (lane & 7) ^ ((lr >> 1) & 7);
+      const char* base;
+      int64_t end;
+      unsigned v;
+      if (j < 2 * S) {
+        const int first = n0 + (GATED ? j % S * 8 : j * 8);  // S copies of gate, then of up
+        base = g.b[GATED && j >= S ? 1 : 0] + first * g.ldb + (int64_t)k * ES;
+        end = (g.N - 1 - first) * g.ldb + chunked((int64_t)g.K * ES) - (int64_t)k * ES;
+        v = (unsigned)((lane >> 3) * g.ldb);
+      } else {
+        const int first = (j - 2 * S) * 8;
+        base = g.a[0] + first * g.lda + (int64_t)k * ES;
+        end = (g.M - 1 - first) * g.lda + chunked((int64_t)g.K * ES) - (int64_t)k * ES;
+        v = (unsigned)((lane >> 3) * g.lda);
+      }
+      const int records = !live || end < 0 ? 0 : end > 0x7fffffff ? 0x7fffffff : (int)end;
+      const __amdgpu_buffer_rsrc_t src =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, records, 0x00020000);
+      v = chunk * EPC < g.K - k ? v + chunk * 16 : kOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          src, (__attribute__((address_space(3))) void*)(slot + j * 1024), 16, (int)v, 0, 0, 0);
+    }
+  };
+
+  const int steps = (g.K + KB - 1) / KB, per = (steps + waves - 1) / waves;
+  const int s0 = wave * per, s1 = min(steps, s0 + per);
+  Acc acc[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) acc[i] = Acc{};
+#pragma unroll
+  for (int i = 0; i < kRowSlots - 1; ++i) copy(s0 + i, ring + i * SLOT, s0 + i < s1);
+  int at = 0, fill = kRowSlots - 1;
+  for (int s = s0; s < s1; ++s) {
+    copy(s + kRowSlots - 1, ring + fill * SLOT, s + kRowSlots - 1 < s1);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kRowSlots - 1) * COPIES) : "memory");
+    const char* const slot = ring + at * SLOT;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const int pos = r * kStepBytes + ((kk * 4 + q) ^ ((r >> 1) & 7)) * 16;
+      const u32x4 a = lds_b128(slot + 2 * S * 1024 + pos);
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        acc[i] = Mma<T>::add(lds_b128(slot + i * 2048 + pos), a, acc[i]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next copy replaces it
+    at = at + 1 == kRowSlots ? 0 : at + 1;
+    fill = fill + 1 == kRowSlots ? 0 : fill + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  join_waves<T, S, EPI>(g, acc, smem, n0, wave, waves, lane);
+}
+
+// k_dense_any: the same for rows that are no whole 16-byte chunks, with loads straight
+// into the products' registers: 16 bytes of one row a lane, of any alignment.  Rows past
+// the matrices' ends read the last one again, their results are dropped.
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+
+// 16 bytes at element k of a row of K elements, zero behind its end.
+template <typename T>
+__device__ __forceinline__ u32x4 load_tail(const char* row, int k, int K) {
+  constexpr int N = 16 / sizeof(T);
+  typedef typename std::conditional<sizeof(T) == 1, uint8_t,
+                                    typename std::conditional<sizeof(T) == 2, uint16_t,
+                                                              uint32_t>::type>::type U;
+  typedef U V __attribute__((ext_vector_type(N)));
+  V v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = k + i < K ? ((const U*)row)[k + i] : (U)0;
+  return __builtin_bit_cast(u32x4, v);
+}
+
+template <typename T, int EPI>
+__global__ __launch_bounds__(512) void k_dense_any(GemmArgs g) {
+  constexpr bool GATED = EPI == kGated || EPI == kGatedMax;
+  constexpr int KB = kStepBytes / 2 / sizeof(T), EPC = 16 / sizeof(T);
+  constexpr int kUnroll = 8;
+  typedef typename Mma<T>::Acc Acc;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int n0 = blockIdx.x * (GATED ? 8 : 16);
+  const int row = min(n0 + (GATED ? r & 7 : r), g.N - 1);
+  const char* const pb = g.b[GATED ? r >> 3 : 0] + row * g.ldb;
+  const char* const pa = g.a[0] + min(r, g.M - 1) * g.lda;
+
+  // 64-byte stages of K in whole 128-byte pairs per wave.
+  const int stages = (g.K + KB - 1) / KB, per = (stages + 2 * waves - 1) / (2 * waves) * 2;
+  const int whole = g.K / KB;  // stages without a tail
+  int s = min(stages, wave * per);
+  const int end = min(stages, s + per);
+  Acc acc[1] = {};
+  auto run = [&](auto count) {  // `count` stages without a tail
+    constexpr int U = decltype(count)::value;
+    u32x4 b[U], a[U];
+    const int64_t at = (int64_t)s * 64 + q * 16;
+#pragma unroll
+    for (int j = 0; j < U; ++j) b[j] = *(const u32x4_any*)(pb + at + j * 64);
+#pragma unroll
+    for (int j = 0; j < U; ++j) a[j] = *(const u32x4_any*)(pa + at + j * 64);
+#pragma unroll
+    for (int j = 0; j < U; ++j) acc[0] = Mma<T>::add(b[j], a[j], acc[0]);
+    s += U;
+  };
+  const int fast = min(end, whole);
+  while (s + kUnroll <= fast) run(std::integral_constant<int, kUnroll>{});
+  if (s + kUnroll / 2 <= fast) run(std::integral_constant<int, kUnroll / 2>{});
+  if (s + kUnroll / 4 <= fast) run(std::integral_constant<int, kUnroll / 4>{});
+  while (s < fast) run(std::integral_constant<int, 1>{});
+  for (; s < end; ++s) {
+    const int k = s * KB + q * EPC;
+    acc[0] = Mma<T>::add(load_tail<T>(pb, k, g.K), load_tail<T>(pa, k, g.K), acc[0]);
+  }
+  join_waves<T, 1, EPI>(g, acc, smem, n0, wave, waves, lane);
+}
+
 // ---- launching --------------------------------------------------------------
-template <typename T, int WM, int WN, int MT, int G, bool AS, bool BS, int EPI>
+template <typename T, int WM, int WN, int MT, int G, int SLOTS, bool AS, bool BS, int EPI>
 hipError_t launch_tile(const GemmArgs& g, hipStream_t s) {
-  const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.nprob * g.slices;
-  k_dense<T, WM, WN, MT, G, AS, BS, EPI><<<(unsigned)blocks, WM * WN * 64, 0, s>>>(g);
+  const int tail = g.tiles - g.whole;
+  const int64_t blocks = g.whole + (int64_t)tail * g.slices;
+  k_dense<T, WM, WN, MT, G, SLOTS, AS, BS, EPI><<<(unsigned)blocks, WM * WN * 64, 0, s>>>(g);
+  if (tail > 0) {
+    const int64_t waves = (int64_t)tail * WM * WN * G * MT;
+    k_dense_join<T, WM, WN, MT, G, BS, EPI><<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(g);
+  }
+  return hipGetLastError();
+}
+
+template <typename T, int EPI>
+hipError_t launch_rows(const GemmArgs& g, int shape, hipStream_t s) {
+  const unsigned blocks = (unsigned)g.tiles;
+  const int waves = g.slices;
+  if (shape == kRowsAny)
+    k_dense_any<T, EPI><<<blocks, waves * 64, waves * 1024, s>>>(g);
+  else if (shape == kRows16)
+    k_dense_rows<T, 1, EPI><<<blocks, waves * 64, waves * kRowSlots * 4096, s>>>(g);
+  else
+    k_dense_rows<T, 2, EPI><<<blocks, waves * 64, waves * kRowSlots * 6144, s>>>(g);
   return hipGetLastError();
 }
 
 template <typename T, bool AS, bool BS, int EPI>
 hipError_t launch_shape(const GemmArgs& g, int shape, hipStream_t s) {
   switch (shape) {
+    case kRows16:
+    case kRows32:
+    case kRowsAny:
+      if constexpr (!AS && !BS && EPI != kGateGrad) return launch_rows<T, EPI>(g, shape, s);
+      return hipErrorInvalidValue;
     case kTile256:  // fp32 is bound by its products, not by the LDS: smaller wave tiles
-      if constexpr (sizeof(T) == 4) return launch_tile<T, 2, 4, 8, 1, AS, BS, EPI>(g, s);
-      return launch_tile<T, 2, 2, 8, 2, AS, BS, EPI>(g, s);
-    case kTile128: return launch_tile<T, 2, 2, 4, 1, AS, BS, EPI>(g, s);
-    default: return launch_tile<T, 1, 4, 4, 1, AS, BS, EPI>(g, s);
+      if constexpr (sizeof(T) == 4) return launch_tile<T, 2, 4, 8, 1, 2, AS, BS, EPI>(g, s);
+      else return launch_tile<T, 2, 2, 8, 2, 2, AS, BS, EPI>(g, s);
+    case kTile128: return launch_tile<T, 2, 2, 4, 1, 2, AS, BS, EPI>(g, s);
+    default: return launch_tile<T, 1, 4, 4, 1, 2, AS, BS, EPI>(g, s);
   }
-}
-
-// EPI of the whole product; SPLIT the epilogue of its slices.
-template <typename T, bool AS, bool BS, int EPI, int SPLIT>
-hipError_t launch_epi(const GemmArgs& g, int shape, hipStream_t s) {
-  if (g.slices == 1) return launch_shape<T, AS, BS, EPI>(g, shape, s);
-  const hipError_t e = launch_shape<T, AS, BS, SPLIT>(g, shape, s);
-  if (e != hipSuccess) return e;
-  const int64_t rows = (int64_t)g.M * g.nprob;
-  const dim3 grid((g.N + 1023) / 1024, (unsigned)(rows < 65535 ? rows : 65535));
-  k_dense_join<T, EPI><<<grid, 256, 0, s>>>(g);
-  return hipGetLastError();
 }
 
 // The products of a floating-point type.
 template <typename T>
 hipError_t launch_float(const GemmArgs& g, int shape, int form, hipStream_t s) {
   switch (form) {
-    case kFormGated: return launch_epi<T, false, false, kGated, kPartGated>(g, shape, s);
-    case kFormKcKc: return launch_epi<T, false, false, kStore, kPart>(g, shape, s);
-    case kFormGateGrad: return launch_epi<T, false, true, kGateGrad, kPart>(g, shape, s);
-    case kFormKcKs: return launch_epi<T, false, true, kStore, kPart>(g, shape, s);
-    default: return launch_epi<T, true, true, kStore, kPart>(g, shape, s);
+    case kFormGated: return launch_shape<T, false, false, kGated>(g, shape, s);
+    case kFormKcKc: return launch_shape<T, false, false, kStore>(g, shape, s);
+    case kFormGateGrad: return launch_shape<T, false, true, kGateGrad>(g, shape, s);
+    case kFormKcKs: return launch_shape<T, false, true, kStore>(g, shape, s);
+    default: return launch_shape<T, true, true, kStore>(g, shape, s);
   }
 }
 

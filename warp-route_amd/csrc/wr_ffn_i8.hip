@@ -7,8 +7,8 @@ namespace ffn {
 
 hipError_t launch_i8(const GemmArgs& g, int shape, int form, hipStream_t s) {
   if (form == kFormGatedMax)
-    return launch_epi<int8_t, false, false, kGatedMax, kPartGated>(g, shape, s);
-  return launch_epi<int8_t, false, false, kScale, kPart>(g, shape, s);
+    return launch_shape<int8_t, false, false, kGatedMax>(g, shape, s);
+  return launch_shape<int8_t, false, false, kScale>(g, shape, s);
 }
 
 }  // namespace ffn
