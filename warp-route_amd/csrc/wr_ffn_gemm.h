@@ -15,7 +15,7 @@
 //
 // Tiles.  A K step is 128 bytes of K: 64 16-bit elements, 128 int8, 32 fp32.
 // Both operand tiles of a step are copied from memory straight into LDS
-// (buffer_load ... lds, 16 bytes a lane), into a ring of 2 or 4 buffers of which
+// (buffer_load ... lds, 16 bytes a lane), into a ring of 2 or 3 buffers of which
 // one is multiplied.  The copy's buffer descriptor ends at the operand's
 // last element, so rows past the end arrive as zeros without a branch; K
 // tails and column tails give their lanes an offset behind the descriptor.
@@ -151,41 +151,44 @@ struct TileCopy {
     return (lane & 7) ^ kc_key<NSIDE>(row);
   }
 
-  // cols: KS only, m (n) elements left from the tile's first one.
-  __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int cols) {
+  // left: elements left from the tile's first one, of m (n) (KS) or of K (KC: KB or more
+  // except at the last step of a segment).
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int left) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
+      int c;  // chunk of this lane in its row
+      unsigned at;
       if (KS) {
         constexpr int CPR = ROWS * ES / 16;  // chunks per k row
         const int L = (j * NW + wave) * 64 + lane;
         const int k = L / CPR, p = L % CPR;
-        constexpr int G = ES == 4 ? 4 : 2;  // chunks per swizzle unit
-        const int c = ((p / G) ^ ks_key<ES, ROWS>(k)) * G + p % G;
-        voff[j] = c * EPC < cols ? (unsigned)(k * ld + c * 16) : kOutside;
+        constexpr int U = ES == 4 ? 4 : 2;  // chunks per swizzle unit
+        c = ((p / U) ^ ks_key<ES, ROWS>(k)) * U + p % U;
+        at = (unsigned)(k * ld);
       } else {
         int row = (j * NW + wave) * 8 + (lane >> 3);
+        c = (lane & 7) ^ kc_key<NSIDE>(row);
         if (GATED) row = (row >> 4) * 8 + (row & 7);  // rows 8..15 of 16 are the other matrix's
-        voff[j] = (unsigned)(row * ld + k_chunk(j, wave, lane) * 16);
+        at = (unsigned)(row * ld);
       }
+      voff[j] = c * EPC < left ? at + c * 16 : kOutside;
     }
   }
 
-  // base: the tile's first byte at this K step; end: the operand's bytes from there
-  // on (<= 0: the step does not exist, zeros arrive).
-  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(const char* base, int64_t end) {
-    const int records = end > 0x7fffffff ? 0x7fffffff : end < 0 ? 0 : (int)end;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, records, 0x00020000);
-  }
-  // Copy j; krem: K elements left at this step.
-  __device__ __forceinline__ void issue(int j, char* lds, __amdgpu_buffer_rsrc_t r, int krem,
-                                        int wave, int lane) const {
-    unsigned v = voff[j];
-    if (!KS) v = k_chunk(j, wave, lane) * EPC < krem ? v : kOutside;
+  // Copy j from a descriptor whose base is the tile's first byte at this K step.
+  __device__ __forceinline__ void issue(int j, char* lds, __amdgpu_buffer_rsrc_t r, int wave) const {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        r, (__attribute__((address_space(3))) void*)(lds + (j * NW + wave) * 1024), 16, (int)v, 0,
-        0, 0);
+        r, (__attribute__((address_space(3))) void*)(lds + (j * NW + wave) * 1024), 16,
+        (int)voff[j], 0, 0, 0);
   }
 };
+
+// Descriptor of the `end` bytes from base (none: every lane's copy is zero).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const char* base, int64_t end) {
+  const int high = (int)(end >> 31);
+  const int records = high == 0 ? (int)end : high < 0 ? 0 : 0x7fffffff;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, records, 0x00020000);
+}
 
 // ---- reading a wave's fragments from LDS -----------------------------------
 __device__ __forceinline__ u32x4 lds_b128(const char* p) {
@@ -460,36 +463,59 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
   typedef TileCopy<T, BN, NW, BS, true, GATED> CopyB;
   CopyA ca;
   CopyB cb;
-  ca.init(wave, lane, g.lda, AS ? g.M - m0 : 0);
-  cb.init(wave, lane, g.ldb, BS ? g.N - n0 : 0);
   Frag<T, BM, MT, AS, false> fa;
   Frag<T, BN, NT, BS, true> fb;
   fa.init(wm * MT, lane);
   fb.init(wn * NT, lane);
 
-  const char* const pa0 = g.a[id.prob];
-  const char* const pa1 = g.a[1];
-  const char* const pb0 = g.b[GATED ? (wave & 1) : 0];
-  const char* const pb1 = g.b[1];
-  // Where a step's tiles come from.
+  // The next step to copy: its first bytes, the operands' bytes from there on, its K
+  // elements left.
+  const int seg0 = s0 >= steps ? 1 : 0, k0 = (s0 - seg0 * steps) * KB;
+  const int64_t stepa = AS ? KB * g.lda : kStepBytes, stepb = BS ? KB * g.ldb : kStepBytes;
+  const int64_t offa = AS ? (int64_t)m0 * ES : m0 * g.lda, offb = BS ? (int64_t)n0 * ES : n0 * g.ldb;
+  const int64_t alla = AS ? (g.K - 1) * g.lda + chunked((int64_t)g.M * ES)
+                          : (g.M - 1) * g.lda + chunked((int64_t)g.K * ES);
+  const int64_t allb = BS ? (g.K - 1) * g.ldb + chunked((int64_t)g.N * ES)
+                          : (g.N - 1) * g.ldb + chunked((int64_t)g.K * ES);
+  const char* const pa1 = g.a[1] + offa;
+  const char* const pb1 = g.b[1] + offb;
+  const char* pa = (seg0 ? pa1 : g.a[id.prob] + offa) + (s0 - seg0 * steps) * stepa;
+  const char* pb = (seg0 ? pb1 : g.b[GATED ? (wave & 1) : 0] + offb) + (s0 - seg0 * steps) * stepb;
+  int64_t enda = alla - offa - (s0 - seg0 * steps) * stepa;
+  int64_t endb = allb - offb - (s0 - seg0 * steps) * stepb;
+  int krem = g.K - k0, todo = s1 - s0;
+  auto offsets = [&]() {
+    ca.init(wave, lane, g.lda, AS ? g.M - m0 : krem);
+    cb.init(wave, lane, g.ldb, BS ? g.N - n0 : krem);
+  };
+  offsets();
   struct Source {
     __amdgpu_buffer_rsrc_t a, b;
-    int krem;
   };
-  auto source = [&](int step) {
-    const int seg = step >= steps ? 1 : 0;
-    const int k = (step - seg * steps) * KB;
-    const bool live = step < s1;
-    const char* pa = seg ? pa1 : pa0;
-    const int64_t offa = AS ? k * g.lda + (int64_t)m0 * ES : m0 * g.lda + (int64_t)k * ES;
-    const int64_t alla = AS ? (g.K - 1) * g.lda + chunked((int64_t)g.M * ES)
-                            : (g.M - 1) * g.lda + chunked((int64_t)g.K * ES);
-    const char* pb = seg ? pb1 : pb0;
-    const int64_t offb = BS ? k * g.ldb + (int64_t)n0 * ES : n0 * g.ldb + (int64_t)k * ES;
-    const int64_t allb = BS ? (g.K - 1) * g.ldb + chunked((int64_t)g.N * ES)
-                            : (g.N - 1) * g.ldb + chunked((int64_t)g.K * ES);
-    return Source{CopyA::source(pa + offa, live ? alla - offa : 0),
-                  CopyB::source(pb + offb, live ? allb - offb : 0), g.K - k};
+  // The step's descriptors; a step that does not exist (todo <= 0) copies zeros.
+  auto source = [&]() {
+    const Source r{descriptor(pa, todo > 0 ? enda : 0), descriptor(pb, todo > 0 ? endb : 0)};
+    return r;
+  };
+  // On to the next one.  The lanes' offsets change only around a segment's last step, whose
+  // chunks past K they leave out.
+  auto advance = [&]() {
+    --todo;
+    pa += stepa;
+    pb += stepb;
+    enda -= stepa;
+    endb -= stepb;
+    krem -= KB;
+    if (krem < KB) {
+      if (krem <= 0) {
+        pa = pa1;
+        pb = pb1;
+        enda = alla - offa;
+        endb = allb - offb;
+        krem = g.K;
+      }
+      offsets();
+    }
   };
   // Copies lo .. hi - 1 of a step's CopyA::PER + CopyB::PER.
   auto copy = [&](const Source& s, char* lds, int lo, int hi) {
@@ -497,9 +523,9 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
     for (int j = 0; j < CopyA::PER + CopyB::PER; ++j) {
       if (j < lo || j >= hi) continue;
       if (j < CopyA::PER)
-        ca.issue(j, lds, s.a, s.krem, wave, lane);
+        ca.issue(j, lds, s.a, wave);
       else
-        cb.issue(j - CopyA::PER, lds + ABYTES, s.b, s.krem, wave, lane);
+        cb.issue(j - CopyA::PER, lds + ABYTES, s.b, wave);
     }
   };
   constexpr int COPIES = CopyA::PER + CopyB::PER;
@@ -529,7 +555,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
   constexpr int CPG = (COPIES + MT - 1) / MT;
 
 #pragma unroll
-  for (int i = 0; i < SLOTS; ++i) copy(source(s0 + i), smem + i * BUF, 0, COPIES);
+  for (int i = 0; i < SLOTS; ++i) {
+    copy(source(), smem + i * BUF, 0, COPIES);
+    advance();
+  }
   wait_copies<(SLOTS - 1) * COPIES>();
   read(a0, b0, smem, 0, 0, MT + NT);
   settle(acc);
@@ -538,7 +567,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
   // around the loop the sums stay in their registers.
   int s = s0;
   do {
-    const Source after = source(s + SLOTS);
+    const Source after = source();
     char* const cur = smem + at * BUF;
     at = at + 1 == SLOTS ? 0 : at + 1;
     char* const next = smem + at * BUF;
@@ -558,6 +587,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
       multiply(a1[i], b1, i);
       __builtin_amdgcn_sched_barrier(0);
     }
+    advance();
   } while (++s < s1);
   wait_copies<0>();
   settle(acc);
@@ -840,7 +870,7 @@ hipError_t launch_shape(const GemmArgs& g, int shape, hipStream_t s) {
       if constexpr (sizeof(T) == 4) return launch_tile<T, 2, 4, 8, 1, 2, AS, BS, EPI>(g, s);
       else return launch_tile<T, 2, 2, 8, 2, 2, AS, BS, EPI>(g, s);
     case kTile128: return launch_tile<T, 2, 2, 4, 1, 2, AS, BS, EPI>(g, s);
-    default: return launch_tile<T, 1, 4, 4, 1, 2, AS, BS, EPI>(g, s);
+    default: return launch_tile<T, 2, 2, 4, 1, 3, AS, BS, EPI>(g, s);
   }
 }
 

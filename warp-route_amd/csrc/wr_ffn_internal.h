@@ -37,8 +37,9 @@ struct GemmArgs {
   bool vec;  // out rows and pointer are 16-byte aligned
 };
 
-// Tile shapes (m x n; gated products: n / 2 columns of each matrix).
-enum Shape { kTile256, kTile128, kTile64, kShapes,  // 256 x 256, 128 x 128, 64 x 256
+// Tile shapes (m x n; gated products: n / 2 columns of each matrix): 256 x 256, 128 x 128,
+// and 128 x 128 with a deeper ring, one block a CU.
+enum Shape { kTile256, kTile128, kTile128Deep, kShapes,
              // few rows: `tiles` blocks of `slices` waves over 16 or 32 rows of B
              kRows16 = kShapes, kRows32, kRowsAny };
 
