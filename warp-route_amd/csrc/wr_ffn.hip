@@ -21,24 +21,36 @@ int elem_bytes(int dtype) { return dtype == WR_F32 ? 4 : 2; }
 bool float_dtype(int d) { return d == WR_F32 || d == WR_F16 || d == WR_BF16; }
 
 // ---- row kernels --------------------------------------------------------------
-// Rows of `bytes` bytes to rows of `ld` bytes, the tail zero: operands whose rows are
-// no whole 16-byte chunks, for the product kernels' 16-byte copies.  Bound by the
-// bytes; a thread assembles one 16-byte chunk from units of U, the element type.
+// Rows of a call's operands to rows of whole 16-byte chunks, the tails zero, for the product
+// kernels' 16-byte copies: all of a call's in one launch, blockIdx.y the matrix.  Bound
+// by the bytes; a thread assembles one chunk from units of U, the element type.
+constexpr int kMaxPads = 5;
+struct Pads {
+  struct {
+    const void* src;
+    char* dst;
+    int64_t rows, ld;  // ld: bytes
+    int cols;
+  } m[kMaxPads];
+  int n;
+};
 template <typename U>
-__global__ __launch_bounds__(256) void k_pad_rows(const U* __restrict__ src, char* __restrict__ dst,
-                                                  int64_t rows, int cols, int64_t ld) {
+__global__ __launch_bounds__(256) void k_pad_rows(Pads pads) {
+  const auto& job = pads.m[blockIdx.y];
   constexpr int N = 16 / sizeof(U);
   typedef U V __attribute__((ext_vector_type(N)));
-  const int64_t per = ld / 16, total = rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / per;
-    const int c = (int)(i % per) * N;
-    const U* p = src + row * cols + c;
-    V v;
+  const int per = (int)(job.ld / 16);
+  // Four rows a block in turn, a wave each.
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < job.rows;
+       row += (int64_t)gridDim.x * 4) {
+    const U* const src = (const U*)job.src + row * job.cols;
+    for (int i = threadIdx.x & 63; i < per; i += 64) {
+      const int c = i * N;
+      V v;
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = c + j < cols ? p[j] : (U)0;
-    *(V*)(dst + i * 16) = v;
+      for (int j = 0; j < N; ++j) v[j] = c + j < job.cols ? src[c + j] : (U)0;
+      *(V*)(job.dst + row * job.ld + i * 16) = v;
+    }
   }
 }
 
@@ -67,90 +79,128 @@ __device__ __forceinline__ int code_of(float x, float m) {
   return (int)rintf(t);
 }
 
-constexpr int kQuantThreads = 256;
+// The scale of a row with maximum m (as fp32 bits).
+__device__ __forceinline__ float scale_of(unsigned mx) {
+  return mx >= 0x7f800000u ? __builtin_nanf("") : mx == 0 ? 1.0f : __uint_as_float(mx) / 127.0f;
+}
 
-// One block per row: max |row|, then the codes (the row's second read comes from
-// cache).  HAVE_MAX: the maxima are there already (as fp32 bits).  codes rows are ldc
-// bytes apart, zero from cols on.  zero_max, when set, gets its word of the row cleared.
-template <typename T, bool HAVE_MAX>
-__global__ __launch_bounds__(kQuantThreads) void k_quantize(const T* __restrict__ x, int64_t ldx,
-                                                            int cols, const unsigned* row_max,
-                                                            int8_t* __restrict__ codes, int64_t ldc,
-                                                            float* __restrict__ scales,
-                                                            unsigned* __restrict__ zero_max,
-                                                            bool vec) {
-  __shared__ unsigned part[kQuantThreads / 64];
+constexpr int kQuantHeld = 4;  // vectors of a row that a thread keeps from the maximum to the codes
+
+// One block per row: max |row|, then the codes; a row's first kQuantHeld vectors per thread
+// stay in registers, what is longer is read again.  codes rows are ldc bytes apart, zero
+// from cols on.  zero_max, when set, gets its word of the row cleared.  VEC: rows are
+// whole 16-byte vectors.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(1024) void k_quantize(const T* __restrict__ x, int cols,
+                                                   int8_t* __restrict__ codes, int64_t ldc,
+                                                   float* __restrict__ scales,
+                                                   unsigned* __restrict__ zero_max) {
+  __shared__ unsigned part[16];
   const int64_t row = blockIdx.x;
-  const T* p = x + row * ldx;
-  constexpr int N = 16 / sizeof(T);
+  const T* p = x + row * cols;
+  constexpr int N = VEC ? 16 / sizeof(T) : 1;
   typedef T V __attribute__((ext_vector_type(N)));
+  typedef int8_t Q __attribute__((ext_vector_type(N)));
+  const int step = blockDim.x * N;
+  auto top = [](V v) {
+    unsigned mx = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) mx = max(mx, __float_as_uint(as_float(v[i])) & 0x7fffffffu);
+    return mx;
+  };
+  V held[kQuantHeld];
   unsigned mx = 0;
-  if (HAVE_MAX) {
-    mx = row_max[row];
-  } else {
-    if (vec) {
-      for (int c = threadIdx.x * N; c < cols; c += kQuantThreads * N) {
-        const V v = *(const V*)(p + c);
 #pragma unroll
-        for (int i = 0; i < N; ++i) mx = max(mx, __float_as_uint(as_float(v[i])) & 0x7fffffffu);
-      }
-    } else {
-      for (int c = threadIdx.x; c < cols; c += kQuantThreads)
-        mx = max(mx, __float_as_uint(as_float(p[c])) & 0x7fffffffu);
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) mx = max(mx, (unsigned)__shfl_xor((int)mx, d));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kQuantThreads / 64; ++i) mx = max(mx, part[i]);
+  for (int j = 0; j < kQuantHeld; ++j) {
+    const int c = threadIdx.x * N + j * step;
+    held[j] = V{};
+    if (c < cols) held[j] = *(const V*)(p + c);
   }
-  const bool finite = mx < 0x7f800000u;
-  const float m = __uint_as_float(mx);
+#pragma unroll
+  for (int j = 0; j < kQuantHeld; ++j) mx = max(mx, top(held[j]));
+  for (int c = threadIdx.x * N + kQuantHeld * step; c < cols; c += step)
+    mx = max(mx, top(*(const V*)(p + c)));
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) mx = max(mx, (unsigned)__shfl_xor((int)mx, d));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
+  __syncthreads();
+  for (int i = 0; i < (int)blockDim.x / 64; ++i) mx = max(mx, part[i]);
   if (threadIdx.x == 0) {
-    scales[row] = !finite ? __builtin_nanf("") : mx == 0 ? 1.0f : m / 127.0f;
+    scales[row] = scale_of(mx);
     if (zero_max != nullptr) zero_max[row] = 0;
   }
-  const bool live = finite && mx != 0;
-  int8_t* q = codes + row * ldc;
-  typedef int8_t Q __attribute__((ext_vector_type(N)));
-  if (vec && ldc % N == 0) {
-    for (int c = threadIdx.x * N; c < (int)ldc; c += kQuantThreads * N) {
-      Q o;
-      if (c < cols) {
-        const V v = *(const V*)(p + c);
+  const bool live = mx < 0x7f800000u && mx != 0;
+  const float m = __uint_as_float(mx);
+  int8_t* const q = codes + row * ldc;
+  auto code = [&](int c, V v) {
+    Q o;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          o[i] = live && c + i < cols ? (int8_t)code_of(as_float(v[i]), m) : (int8_t)0;
-      } else {
-        o = Q{};
-      }
-      *(Q*)(q + c) = o;
+    for (int i = 0; i < N; ++i) o[i] = live ? (int8_t)code_of(as_float(v[i]), m) : (int8_t)0;
+    *(Q*)(q + c) = o;
+  };
+#pragma unroll
+  for (int j = 0; j < kQuantHeld; ++j) {
+    const int c = threadIdx.x * N + j * step;
+    if (c < cols) code(c, held[j]);
+  }
+  for (int c = threadIdx.x * N + kQuantHeld * step; c < cols; c += step) code(c, *(const V*)(p + c));
+  for (int c = cols + threadIdx.x; c < (int)ldc; c += blockDim.x) q[c] = 0;
+}
+
+// Codes of fp32 rows whose maxima are known, 4 columns a thread: rows of ldx elements to
+// rows of ldx codes, zero from cols on.
+__global__ __launch_bounds__(256) void k_quantize_known(const float* __restrict__ x, int64_t ldx,
+                                                        int rows, int cols,
+                                                        const unsigned* __restrict__ row_max,
+                                                        int8_t* __restrict__ codes,
+                                                        float* __restrict__ scales) {
+  typedef int8_t Q __attribute__((ext_vector_type(4)));
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (c >= ldx) return;
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    const unsigned mx = row_max[row];
+    if (c == 0) scales[row] = scale_of(mx);
+    Q o{};
+    if (mx < 0x7f800000u && mx != 0 && c < cols) {
+      const f32x4 v = *(const f32x4*)(x + row * ldx + c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < cols) o[i] = (int8_t)code_of(v[i], __uint_as_float(mx));
     }
-  } else {
-    for (int c = threadIdx.x; c < (int)ldc; c += kQuantThreads)
-      q[c] = live && c < cols ? (int8_t)code_of(as_float(p[c]), m) : (int8_t)0;
+    *(Q*)(codes + row * ldx + c) = o;
   }
 }
 
-template <bool HAVE_MAX>
-hipError_t launch_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols,
-                           const unsigned* row_max, int8_t* codes, int64_t ldc, float* scales,
-                           unsigned* zero_max, hipStream_t s) {
-  if (rows == 0) return hipSuccess;
-  const int n = 16 / elem_bytes(dtype);
-  // Vector reads may pass cols inside a row's padding, never the row.
-  const bool vec = ldx % n == 0 && round_up(cols, n) <= ldx &&
-                   reinterpret_cast<uintptr_t>(codes) % 16 == 0;
-  if (dtype == WR_F32)
-    k_quantize<float, HAVE_MAX><<<rows, kQuantThreads, 0, s>>>(
-        (const float*)x, ldx, cols, row_max, codes, ldc, scales, zero_max, vec);
-  else if (dtype == WR_F16)
-    k_quantize<f16, HAVE_MAX><<<rows, kQuantThreads, 0, s>>>((const f16*)x, ldx, cols, row_max,
-                                                             codes, ldc, scales, zero_max, vec);
+template <typename T>
+hipError_t launch_quantize_as(const T* x, int rows, int cols, int8_t* codes, int64_t ldc,
+                              float* scales, unsigned* zero_max, hipStream_t s) {
+  constexpr int N = 16 / sizeof(T);
+  // Two vectors a thread: their latency overlaps, and short rows take few waves.
+  const bool vec = cols % N == 0;
+  const int per = 2 * (vec ? N : 1);
+  const int threads = std::min(1024, std::max(64, (cols + per * 64 - 1) / (per * 64) * 64));
+  if (vec)
+    k_quantize<T, true><<<rows, threads, 0, s>>>(x, cols, codes, ldc, scales, zero_max);
   else
-    k_quantize<__bf16, HAVE_MAX><<<rows, kQuantThreads, 0, s>>>(
-        (const __bf16*)x, ldx, cols, row_max, codes, ldc, scales, zero_max, vec);
+    k_quantize<T, false><<<rows, threads, 0, s>>>(x, cols, codes, ldc, scales, zero_max);
+  return hipGetLastError();
+}
+
+hipError_t launch_quantize(const void* x, int dtype, int rows, int cols, int8_t* codes, int64_t ldc,
+                           float* scales, unsigned* zero_max, hipStream_t s) {
+  if (rows == 0) return hipSuccess;
+  if (dtype == WR_F32)
+    return launch_quantize_as((const float*)x, rows, cols, codes, ldc, scales, zero_max, s);
+  if (dtype == WR_F16)
+    return launch_quantize_as((const f16*)x, rows, cols, codes, ldc, scales, zero_max, s);
+  return launch_quantize_as((const __bf16*)x, rows, cols, codes, ldc, scales, zero_max, s);
+}
+
+hipError_t launch_quantize_known(const float* x, int64_t ldx, int rows, int cols,
+                                 const unsigned* row_max, int8_t* codes, float* scales,
+                                 hipStream_t s) {
+  const dim3 grid((unsigned)((ldx + 1023) / 1024), (unsigned)std::min(rows, 65535));
+  k_quantize_known<<<grid, 256, 0, s>>>(x, ldx, rows, cols, row_max, codes, scales);
   return hipGetLastError();
 }
 
@@ -158,16 +208,14 @@ unsigned row_blocks(int64_t threads) {
   return (unsigned)std::min<int64_t>((threads + 255) / 256, 8192);
 }
 
-hipError_t launch_pad(const void* src, char* dst, int64_t rows, int cols, int64_t ld, int es,
-                      hipStream_t s) {
-  const unsigned blocks = row_blocks(rows * (ld / 16));
-  if (blocks == 0) return hipSuccess;
-  if (es == 4)
-    k_pad_rows<uint32_t><<<blocks, 256, 0, s>>>((const uint32_t*)src, dst, rows, cols, ld);
-  else if (es == 2)
-    k_pad_rows<uint16_t><<<blocks, 256, 0, s>>>((const uint16_t*)src, dst, rows, cols, ld);
-  else
-    k_pad_rows<uint8_t><<<blocks, 256, 0, s>>>((const uint8_t*)src, dst, rows, cols, ld);
+hipError_t launch_pads(const Pads& p, int es, hipStream_t s) {
+  int64_t rows = 0;
+  for (int i = 0; i < p.n; ++i) rows = std::max(rows, p.m[i].rows);
+  if (rows == 0) return hipSuccess;
+  const dim3 grid((unsigned)std::min<int64_t>((rows + 3) / 4, 4096), p.n);
+  if (es == 4) k_pad_rows<uint32_t><<<grid, 256, 0, s>>>(p);
+  else if (es == 2) k_pad_rows<uint16_t><<<grid, 256, 0, s>>>(p);
+  else k_pad_rows<uint8_t><<<grid, 256, 0, s>>>(p);
   return hipGetLastError();
 }
 
@@ -265,6 +313,7 @@ struct Call {
   int dtype;  // of the products' operands, unless int8
   bool int8;
   size_t used = 0, part_at = 0, part_bytes = 0;
+  Pads pads{};
   hipError_t err = hipSuccess;
 
   bool dry() const { return ws == nullptr; }
@@ -279,8 +328,8 @@ struct Call {
   }
   bool go() const { return !dry() && err == hipSuccess; }
 
-  // An operand matrix with whole 16-byte rows: itself, or a padded copy.  any_row: the
-  // product takes rows of any length.
+  // An operand matrix with whole 16-byte rows: itself, or a padded copy, which pad()
+  // makes.  any_row: the product takes rows of any length.
   struct Mat {
     const char* p;
     int64_t ld;  // bytes
@@ -289,8 +338,11 @@ struct Call {
     const int64_t bytes = (int64_t)cols * es(), ld = round_up(bytes, 16);
     if (any_row || ld == bytes) return {(const char*)p, bytes};
     char* c = take(rows * ld);
-    if (go()) check(launch_pad(p, c, rows, cols, ld, es(), stream));
+    pads.m[pads.n++] = {p, c, rows, ld, cols};
     return {c, ld};
+  }
+  void pad() {
+    if (go() && pads.n > 0) check(launch_pads(pads, es(), stream));
   }
 
   // The slices' sums share one region (products of a call run one after another).
@@ -341,6 +393,7 @@ void run_forward(Call& c, const wr_ffn_args& a) {
   const Call::Mat x = c.rows16(a.x, T, h, few);
   const Call::Mat wg = c.rows16(a.w_gate, I, h, few), wu = c.rows16(a.w_up, I, h, few);
   const Call::Mat wd = c.rows16(a.w_down, h, I, few);
+  c.pad();
   char* own = c.take((int64_t)T * Ip * c.es());  // sized whether saved or not
   const Call::Mat act{keep ? (const char*)a.saved_act : own, Ip * c.es()};
 
@@ -362,12 +415,17 @@ void run_backward(Call& c, const wr_ffn_args& a, bool dx, bool dwg, bool dwu, bo
   const int T = a.batch_size, h = a.hidden_dim, I = a.intermediate_dim;
   const int64_t Ip = round_up(I, 64), ldi = Ip * c.es();
   const bool din = dx || dwg || dwu;
+  const Call::Mat none{nullptr, 0};
   const Call::Mat dy = c.rows16(a.dout, T, h);
+  const Call::Mat wd = din ? c.rows16(a.w_down, h, I) : none;
+  const Call::Mat wg = dx ? c.rows16(a.w_gate, I, h) : none;
+  const Call::Mat wu = dx ? c.rows16(a.w_up, I, h) : none;
+  const Call::Mat x = dwg || dwu ? c.rows16(a.x, T, h) : none;
+  c.pad();
   GemmArgs g;
   if (din) {
     char* dgate = c.take(T * ldi);
     char* dup = c.take(T * ldi);
-    const Call::Mat wd = c.rows16(a.w_down, h, I);
     g = gemm(dy, wd, T, I, h);
     g.ldi = Ip;
     g.in[0] = a.saved_gate;
@@ -376,7 +434,6 @@ void run_backward(Call& c, const wr_ffn_args& a, bool dx, bool dwg, bool dwu, bo
     g.out[1] = dup;
     c.product(g, kFormGateGrad);
     if (dx) {
-      const Call::Mat wg = c.rows16(a.w_gate, I, h), wu = c.rows16(a.w_up, I, h);
       g = gemm({dgate, ldi}, wg, T, h, I);
       g.a[1] = dup;
       g.b[1] = wu.p;
@@ -386,7 +443,6 @@ void run_backward(Call& c, const wr_ffn_args& a, bool dx, bool dwg, bool dwu, bo
       c.product(g, kFormKcKs);
     }
     if (dwg || dwu) {
-      const Call::Mat x = c.rows16(a.x, T, h);
       g = gemm({dwg ? dgate : dup, ldi}, x, I, h, T);
       g.a[1] = dup;
       g.nprob = dwg && dwu ? 2 : 1;
@@ -408,6 +464,7 @@ void run_int8(Call& c, const wr_int8_args& a) {
   const bool few = a.rows <= kRowsMax;
   const Call::Mat x = c.rows16(a.x, a.rows, a.in_features, few);
   const Call::Mat w = c.rows16(a.w, a.out_features, a.in_features, few);
+  c.pad();
   GemmArgs g = gemm(x, w, a.rows, a.out_features, a.in_features);
   g.out[0] = a.out;
   g.ldo = a.out_features;
@@ -429,8 +486,9 @@ void run_ffn_int8(Call& c, const wr_ffn_int8_args& a) {
   const bool few = T <= kRowsMax;
   const Call::Mat wg = c.rows16(a.w_gate, I, h, few), wu = c.rows16(a.w_up, I, h, few);
   const Call::Mat wd = c.rows16(a.w_down, h, I, few);
+  c.pad();
   if (c.go())
-    c.check(launch_quantize<false>(a.x, a.dtype, h, T, h, nullptr, xq, hp, sx, amax, c.stream));
+    c.check(launch_quantize(a.x, a.dtype, T, h, xq, hp, sx, amax, c.stream));
   GemmArgs g = gemm({(const char*)xq, hp}, wg, T, I, h);
   g.b[1] = wu.p;
   g.ldi = Ip;
@@ -441,7 +499,7 @@ void run_ffn_int8(Call& c, const wr_ffn_int8_args& a) {
   g.row_max = amax;
   c.product(g, kFormGatedMax);
   if (c.go())
-    c.check(launch_quantize<true>(act, WR_F32, Ip, T, I, amax, aq, Ip, sa, nullptr, c.stream));
+    c.check(launch_quantize_known(act, Ip, T, I, amax, aq, sa, c.stream));
   g = gemm({(const char*)aq, Ip}, wd, T, h, I);
   g.out[0] = a.out;
   g.ldo = h;
@@ -554,8 +612,8 @@ int wr_quantize_int8(const void* x, int dtype, int rows, int cols, int8_t* codes
   if (rows == 0) return WR_OK;
   if (!x || !codes || !scales) return WR_EINVAL_NULL;
   if (!aligned(x) || !aligned(codes) || !aligned(scales)) return WR_EINVAL_ALIGN;
-  return launch_quantize<false>(x, dtype, cols, rows, cols, nullptr, codes, cols, scales, nullptr,
-                                (hipStream_t)stream) == hipSuccess
+  return launch_quantize(x, dtype, rows, cols, codes, cols, scales, nullptr,
+                         (hipStream_t)stream) == hipSuccess
              ? WR_OK
              : WR_EHIP;
 }

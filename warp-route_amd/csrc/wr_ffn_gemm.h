@@ -20,7 +20,7 @@
 // last element, so rows past the end arrive as zeros without a branch; K
 // tails and column tails give their lanes an offset behind the descriptor.
 //
-// A wave owns MT x 4 G tiles of 16 x 16.  B is the MFMA's first operand, so a
+// A wave owns MT x 4 tiles of 16 x 16.  B is the MFMA's first operand, so a
 // lane's four accumulators are four consecutive n of one m.  For KC B the
 // LDS rows of a wave's 64 n are dealt to the MFMA rows so that a lane's 4
 // tiles together hold 16 consecutive n (gated: 8 of gate and the same 8 of
@@ -54,21 +54,11 @@ constexpr int kStepBytes = 128;  // bytes of K per step
 constexpr unsigned kOutside = 0x80000000u;  // offset behind every descriptor
 
 // ---- 16 x 16 tile products over 64 bytes of K --------------------------------
-// The 16-bit and int8 instructions are written as assembly with the sums tied to
-// accumulation registers: the compiler's own register allocation moves the sums of
-// a 128 x 128 wave tile (all 256 accumulation registers) between registers in the
-// loop (add is the compiler's form, for few sums).  The waits its hazard pass would add are held by construction: fragments
-// come from LDS reads alone (no vector instruction writes them), equal sums are at
-// least NT products apart, and settle() stands between the sums' first and last
-// use and any other instruction on them.
 template <typename T>
 struct Mma;
 template <>
 struct Mma<bf16> {
   typedef f32x4 Acc;
-  static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
-    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-  }
   static __device__ __forceinline__ Acc add(u32x4 a, u32x4 b, Acc c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -77,9 +67,6 @@ struct Mma<bf16> {
 template <>
 struct Mma<f16> {
   typedef f32x4 Acc;
-  static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
-    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-  }
   static __device__ __forceinline__ Acc add(u32x4 a, u32x4 b, Acc c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -88,9 +75,6 @@ struct Mma<f16> {
 template <>
 struct Mma<int8_t> {
   typedef i32x4 Acc;
-  static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) {
-    asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-  }
   static __device__ __forceinline__ Acc add(u32x4 a, u32x4 b, Acc c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a),
                                                  __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
@@ -107,19 +91,7 @@ struct Mma<float> {
       c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ void go(u32x4 a, u32x4 b, Acc& c) { c = add(a, b, c); }
 };
-
-// Orders all accumulators' values between the assembly products and other instructions,
-// with the wait states of the longest product (18) in between.
-template <typename Acc, int N>
-__device__ __forceinline__ void settle(Acc (&acc)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+a"(acc[i]));
-  asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+a"(acc[i]));
-}
 
 // ---- copying one operand's K step into LDS ---------------------------------
 // Swizzle keys: KC tiles are [row][128 bytes], KS tiles [k][ROWS elements].
@@ -213,8 +185,7 @@ struct Frag {
   __device__ __forceinline__ void init(int sub0, int lane) {
     const int r = lane & 15, q = lane >> 4;
     if constexpr (!KS) {
-      // M side: row 16 s + r.  N side, per 4 subtiles: subtile t's row r = 4 q' + i is
-      // LDS row 16 q' + 4 t + i.
+      // M side: row 16 s + r.  N side: subtile t's row r = 4 q' + i is LDS row 16 q' + 4 t + i.
       const int row = sub0 * 16 + (NSIDE ? (r >> 2) * 16 + (r & 3) : r);
       const int key = kc_key<NSIDE>(row);
       addr[0] = row * kStepBytes + (q ^ key) * 16;
@@ -236,7 +207,7 @@ struct Frag {
   // Fragment of subtile s, 64-byte half kk of the K step.
   __device__ __forceinline__ u32x4 get(char* tile, int s, int kk) const {
     if constexpr (!KS) {
-      const int row = NSIDE ? (s >> 2) * 64 + (s & 3) * 4 : s * 16;
+      const int row = s * (NSIDE ? 4 : 16);
       return lds_b128(tile + addr[kk] + row * kStepBytes);
     } else if constexpr (ES == 2) {
       typedef __attribute__((address_space(3))) s16x4* P;
@@ -294,12 +265,58 @@ template <typename T, int EPI, bool BS>
 struct Epilogue {
   typedef typename Mma<T>::Acc Acc;
 
+  // What the epilogue of 16 m and 64 n reads, loaded one piece ahead of its use.
+  static constexpr int INS = EPI == kGateGrad ? 8 : EPI == kScale || EPI == kGatedMax ? 4 : 1;
+  struct In {
+    f32x4 v[INS];
+    float row;
+  };
+  // First n of a lane's subtile t.
+  static __device__ __forceinline__ int col(int n0, int q, int t) {
+    return n0 + (BS ? t * 16 + q * 4 : q * 16 + t * 4);
+  }
+  // Four column scales from n, zero past N.
+  static __device__ __forceinline__ f32x4 cols4(const float* p, int n, int N) {
+    typedef f32x4 f32x4_any __attribute__((aligned(4)));
+    f32x4 v{};
+    if (n + 4 <= N) v = *(const f32x4_any*)(p + n);
+    else
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (n + i < N) v[i] = p[n + i];
+    return v;
+  }
+  static __device__ __forceinline__ In load(const GemmArgs& g, int m0, int n0, int lane) {
+    const int q = lane >> 4, m = m0 + (lane & 15);
+    In in{};
+    if (m >= g.M) return in;
+    if constexpr (EPI == kGateGrad) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int n = col(n0, q, t);
+        if (n >= ((g.N + 7) & ~7)) continue;
+        in.v[t] = *(const f32x4*)((const float*)g.in[0] + (int64_t)m * g.ldi + n);
+        in.v[4 + t] = *(const f32x4*)((const float*)g.in[1] + (int64_t)m * g.ldi + n);
+      }
+    } else if constexpr (EPI == kScale) {
+      in.row = g.row_scale[m];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) in.v[t] = cols4(g.col_scale[0], col(n0, q, t), g.N);
+    } else if constexpr (EPI == kGatedMax) {
+      in.row = g.row_scale[m];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        in.v[t] = cols4(g.col_scale[t >> 1], n0 + q * 8 + (t & 1) * 4, g.N);
+    }
+    return in;
+  }
+
   // 16 m from m0, and 64 n from n0 (gated: 32 of gate, 32 of up) in 4 subtiles.
-  static __device__ __forceinline__ void run(const GemmArgs& g, const Acc (&acc)[4], int prob,
-                                             int m0, int n0, int lane) {
+  static __device__ __forceinline__ void run(const GemmArgs& g, const Acc (&acc)[4], const In& in,
+                                             int prob, int m0, int n0, int lane) {
     const int q = lane >> 4, m = m0 + (lane & 15);
     if constexpr (EPI == kGatedMax) {
-      gated_max(g, acc, m, n0 + q * 8);
+      gated_max(g, acc, in, m, n0 + q * 8);
     } else if (m >= g.M) {
       return;
     } else if constexpr (EPI == kGated) {
@@ -310,53 +327,64 @@ struct Epilogue {
         uu[i] = acc[i / 4 + 2][i % 4];
       }
       gated<8>(g, gg, uu, m, n0 + q * 8);
-    } else if constexpr (EPI == kStore && !BS) {
+    } else if constexpr (!BS) {  // 16 consecutive n a lane
       float v[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = acc[i / 4][i % 4];
-      const int n = n0 + q * 16;
-      T* p = (T*)g.out[prob] + (int64_t)m * g.ldo + n;
-      constexpr int V = 16 / sizeof(T);
-#pragma unroll
-      for (int i = 0; i < 16; i += V) store_run<T, V>(p + i, v + i, g.N - n - i, g.vec);
+      for (int i = 0; i < 16; ++i) {
+        v[i] = (float)acc[i / 4][i % 4];
+        if (EPI == kScale) v[i] = v[i] * in.row * in.v[i / 4][i % 4];
+      }
+      store<16>(g, prob, m, n0 + q * 16, v);
     } else {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int n = n0 + (BS ? t * 16 + q * 4 : q * 16 + t * 4);
-        // dg and du rows are read in whole 16-byte chunks: their zeros past N too.
-        if (n < (EPI == kGateGrad ? (g.N + 7) & ~7 : g.N)) tile(g, acc[t], prob, m, n);
+        const int n = col(n0, q, t);
+        if constexpr (EPI == kGateGrad) {
+          // dg and du rows are read in whole 16-byte chunks: their zeros past N too.
+          if (n >= ((g.N + 7) & ~7)) continue;
+          const int64_t at = (int64_t)m * g.ldi + n;
+          float dg[4], du[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            gate_grad(acc[t][i], in.v[t][i], in.v[4 + t][i], dg[i], du[i]);
+          store_run<T, 4>((T*)g.out[0] + at, dg, 4, true);
+          store_run<T, 4>((T*)g.out[1] + at, du, 4, true);
+        } else {
+          tile(g, acc[t], prob, m, n);
+        }
       }
     }
   }
 
+  // C consecutive n of one m into the output.
+  template <typename O, int C>
+  static __device__ __forceinline__ void store_as(const GemmArgs& g, int prob, int m, int n,
+                                                  const float (&v)[C]) {
+    O* const p = (O*)g.out[prob] + (int64_t)m * g.ldo + n;
+    constexpr int V = 16 / sizeof(O) < C ? 16 / sizeof(O) : C;
+#pragma unroll
+    for (int i = 0; i < C; i += V) store_run<O, V>(p + i, v + i, g.N - n - i, g.vec);
+  }
+  template <int C>
+  static __device__ __forceinline__ void store(const GemmArgs& g, int prob, int m, int n,
+                                               const float (&v)[C]) {
+    if constexpr (EPI == kStore) store_as<T>(g, prob, m, n, v);
+    else if (g.out_dtype == WR_F32) store_as<float>(g, prob, m, n, v);
+    else if (g.out_dtype == WR_F16) store_as<f16>(g, prob, m, n, v);
+    else store_as<bf16>(g, prob, m, n, v);
+  }
+
   // Four consecutive n of one m.
   static __device__ __forceinline__ void tile(const GemmArgs& g, Acc a, int prob, int m, int n) {
-    if constexpr (EPI == kStore) {
-      const float v[4] = {a[0], a[1], a[2], a[3]};
-      store_run<T, 4>((T*)g.out[prob] + (int64_t)m * g.ldo + n, v, g.N - n, g.vec);
-    } else if constexpr (EPI == kGateGrad) {
-      const int64_t at = (int64_t)m * g.ldi + n;
-      const f32x4 gg = *(const f32x4*)((const float*)g.in[0] + at);
-      const f32x4 uu = *(const f32x4*)((const float*)g.in[1] + at);
-      float dg[4], du[4];
+    if (m >= g.M || n >= g.N) return;
+    float v[4] = {(float)a[0], (float)a[1], (float)a[2], (float)a[3]};
+    if constexpr (EPI == kScale) {
+      const float row = g.row_scale[m];
+      const f32x4 c = cols4(g.col_scale[0], n, g.N);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) gate_grad(a[i], gg[i], uu[i], dg[i], du[i]);
-      store_run<T, 4>((T*)g.out[0] + at, dg, 4, true);
-      store_run<T, 4>((T*)g.out[1] + at, du, 4, true);
-    } else if constexpr (EPI == kScale) {
-      const float sm = g.row_scale[m];
-      float v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = n + i < g.N ? (float)a[i] * sm * g.col_scale[0][n + i] : 0.0f;
-      const int64_t at = (int64_t)m * g.ldo + n;
-      if (g.out_dtype == WR_F32)
-        store_run<float, 4>((float*)g.out[0] + at, v, g.N - n, g.vec);
-      else if (g.out_dtype == WR_F16)
-        store_run<f16, 4>((f16*)g.out[0] + at, v, g.N - n, g.vec);
-      else
-        store_run<bf16, 4>((bf16*)g.out[0] + at, v, g.N - n, g.vec);
+      for (int i = 0; i < 4; ++i) v[i] = v[i] * row * c[i];
     }
+    store<4>(g, prob, m, n, v);
   }
 
   // C gate and up sums of the same n.  The buffers' rows are padded to ldi (a multiple of
@@ -383,31 +411,27 @@ struct Epilogue {
 
   // int8: a = silu(g) u in fp32 of 8 n from n, with the row maxima of |a| (as fp32 bits: the
   // maximum of non-negative floats is that of their bits, in any order).
-  static __device__ __forceinline__ void gated_max(const GemmArgs& g, const Acc (&acc)[4], int m,
-                                                   int n) {
+  static __device__ __forceinline__ void gated_max(const GemmArgs& g, const Acc (&acc)[4],
+                                                   const In& in, int m, int n) {
     unsigned mx = 0;
     if (m < g.M) {
-      mx = scaled_gate(g, acc[0], acc[2], m, n);
-      mx = max(mx, scaled_gate(g, acc[1], acc[3], m, n + 4));
+      mx = scaled_gate(g, acc[0], acc[2], m, n, in.row, in.v[0], in.v[2]);
+      mx = max(mx, scaled_gate(g, acc[1], acc[3], m, n + 4, in.row, in.v[1], in.v[3]));
     }
     mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
     mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
     if ((threadIdx.x & 63) < 16 && m < g.M) atomicMax(g.row_max + m, mx);
   }
-  // Four n; returns their maximum.
+  // Four n, with the scales of their row and columns (zero past N); returns their maximum.
   static __device__ __forceinline__ unsigned scaled_gate(const GemmArgs& g, Acc gate, Acc up, int m,
-                                                         int n) {
+                                                         int n, float row, f32x4 cg, f32x4 cu) {
     unsigned mx = 0;
     if (n >= g.N) return mx;
-    const float sm = g.row_scale[m];
     float v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[i] = 0.0f;
-      if (n + i < g.N) {
-        const float gg = (float)gate[i] * sm * g.col_scale[0][n + i];
-        v[i] = silu(gg) * ((float)up[i] * sm * g.col_scale[1][n + i]);
-      }
+      v[i] = silu((float)gate[i] * row * cg[i]) * ((float)up[i] * row * cu[i]);
+      if (n + i >= g.N) v[i] = 0.0f;  // a NaN row scale times the zero
       mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
     }
     store_run<float, 4>((float*)g.out[0] + (int64_t)m * g.ldi + n, v, 4, true);
@@ -426,27 +450,28 @@ __device__ __forceinline__ void wait_copies() {
 __device__ __forceinline__ int64_t chunked(int64_t bytes) { return (bytes + 15) & ~(int64_t)15; }
 
 // ---- the kernel -------------------------------------------------------------
-// A block of WM x WN waves, each with MT x 4 G subtiles of 16 x 16.  Both halves' (64
+// A block of WM x WN waves, each with MT x 4 subtiles of 16 x 16.  Both halves' (64
 // bytes of K) fragments are held in registers: while one half is multiplied, the
 // other's are read.  The K step's only barrier lies between its halves: behind it the
 // next step's tiles are in LDS (their copies were issued SLOTS - 1 steps earlier)
 // and nobody reads the present ones any more, which the copies of step s + SLOTS
-// then replace.  Each half is written as MT groups of NT products, with the LDS
+// then replace.  Each half is written as MT groups of 4 products, with the LDS
 // reads and copies dealt to the groups and the groups kept in order, so that
 // the matrix cores, the LDS and the copies run side by side in one wave.
 //
-// 128 x 128 wave tiles (256 x 256, 4 waves) read 128 KB of fragments per K step
-// beside 64 KB of copies: at the LDS's 128 bytes a clock three quarters of the
-// products' 2048 clocks.  8 waves of 128 x 64 read 192 KB, which takes all of them.
-template <typename T, int WM, int WN, int MT, int G, int SLOTS, bool AS, bool BS, int EPI>
-__global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
+// Measured (bf16, 4096 x 14336 by 14336 x 4096): 326 us, 1475 TFLOP/s; with the copies and LDS
+// reads left out the time is the same, so the matrix cores at their clock under load
+// bound the loop.  4 waves of 128 x 128 (all 512 registers) take the same time; tiles of
+// 128 x 128 404 us.  The launch bound and the LDS given at launch keep 4 waves of 64 x
+// 64 to 256 registers: with more the compiler moves sums between register files.
+template <typename T, int WM, int WN, int MT, int SLOTS, bool AS, bool BS, int EPI>
+__global__ __launch_bounds__(WM * WN * 64, 2) void k_dense(GemmArgs g) {
   constexpr bool GATED = EPI == kGated || EPI == kGatedMax;
-  constexpr int NT = 4 * G;
-  constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
+  constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * 64;
   constexpr int ABYTES = BM * kStepBytes, BBYTES = BN * kStepBytes, BUF = ABYTES + BBYTES;
   constexpr int ES = sizeof(T), KB = kStepBytes / ES;
   typedef typename Mma<T>::Acc Acc;
-  __shared__ __attribute__((aligned(1024))) char smem[SLOTS * BUF];
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [SLOTS][BUF]
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -464,9 +489,9 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
   CopyA ca;
   CopyB cb;
   Frag<T, BM, MT, AS, false> fa;
-  Frag<T, BN, NT, BS, true> fb;
+  Frag<T, BN, 4, BS, true> fb;
   fa.init(wm * MT, lane);
-  fb.init(wn * NT, lane);
+  fb.init(wn * 4, lane);
 
   // The next step to copy: its first bytes, the operands' bytes from there on, its K
   // elements left.
@@ -530,28 +555,28 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
   };
   constexpr int COPIES = CopyA::PER + CopyB::PER;
 
-  Acc acc[G * MT * 4];  // [group of 4 n subtiles][m subtile][n subtile]
+  Acc acc[MT * 4];  // [m subtile][n subtile]
 #pragma unroll
-  for (int i = 0; i < G * MT * 4; ++i) acc[i] = Acc{};
+  for (int i = 0; i < MT * 4; ++i) acc[i] = Acc{};
 
-  u32x4 a0[MT], b0[NT], a1[MT], b1[NT];
+  u32x4 a0[MT], b0[4], a1[MT], b1[4];
   // Fragments lo .. hi - 1, those of B first: every product needs them.
-  auto read = [&](u32x4(&a)[MT], u32x4(&b)[NT], char* tile, int kk, int lo, int hi) {
+  auto read = [&](u32x4(&a)[MT], u32x4(&b)[4], char* tile, int kk, int lo, int hi) {
 #pragma unroll
-    for (int j = 0; j < MT + NT; ++j) {
+    for (int j = 0; j < MT + 4; ++j) {
       if (j < lo || j >= hi) continue;
-      if (j < NT)
+      if (j < 4)
         b[j] = fb.get(tile + ABYTES, j, kk);
       else
-        a[j - NT] = fa.get(tile, j - NT, kk);
+        a[j - 4] = fa.get(tile, j - 4, kk);
     }
   };
-  auto multiply = [&](const u32x4& a, const u32x4(&b)[NT], int i) {
+  auto multiply = [&](const u32x4& a, const u32x4(&b)[4], int i) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) Mma<T>::go(b[t], a, acc[((t >> 2) * MT + i) * 4 + (t & 3)]);
+    for (int t = 0; t < 4; ++t) acc[i * 4 + t] = Mma<T>::add(b[t], a, acc[i * 4 + t]);
   };
   // Reads per group: done two groups before the half's end, for their latency.
-  constexpr int RPG = (MT + NT + MT - 3) / (MT - 2);
+  constexpr int RPG = (MT + 4 + MT - 3) / (MT - 2);
   constexpr int CPG = (COPIES + MT - 1) / MT;
 
 #pragma unroll
@@ -560,11 +585,9 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
     advance();
   }
   wait_copies<(SLOTS - 1) * COPIES>();
-  read(a0, b0, smem, 0, 0, MT + NT);
-  settle(acc);
+  read(a0, b0, smem, 0, 0, MT + 4);
   int at = 0;
-  // An empty slice runs one step of zeros (no step of it is live): without a way
-  // around the loop the sums stay in their registers.
+  // An empty slice runs one step of zeros (no step of it exists).
   int s = s0;
   do {
     const Source after = source();
@@ -590,49 +613,68 @@ __global__ __launch_bounds__(WM * WN * 64) void k_dense(GemmArgs g) {
     advance();
   } while (++s < s1);
   wait_copies<0>();
-  settle(acc);
   // A slice stores its sums as they lie in the registers.
   Acc* const part = id.tail < 0 ? nullptr
                                 : (Acc*)g.part + ((int64_t)(id.tail * g.slices + id.slice) * NW + wave) *
-                                                     (G * MT * 4 * 64) + lane;
+                                                     (MT * 4 * 64) + lane;
+  typedef Epilogue<T, EPI, BS> E;
+  // Pieces of 16 m x 64 n.
+  auto pm = [&](int p) { return m0 + (wm * MT + p) * 16; };
+  const int pn = n0 + wn * (GATED ? 32 : 64);
+  typename E::In in{};
+  if (part == nullptr) in = E::load(g, pm(0), pn, lane);
 #pragma unroll
-  for (int j = 0; j < G; ++j)
+  for (int p = 0; p < MT; ++p) {
+    const Acc(&piece)[4] = *reinterpret_cast<Acc(*)[4]>(&acc[p * 4]);
+    if (part == nullptr) {
+      typename E::In next{};
+      if (p + 1 < MT) next = E::load(g, pm(p + 1), pn, lane);
+      E::run(g, piece, in, id.prob, pm(p), pn, lane);
+      in = next;
+    } else if (pm(p) < g.M) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const Acc(&piece)[4] = *reinterpret_cast<Acc(*)[4]>(&acc[(j * MT + i) * 4]);
-      const int m = m0 + (wm * MT + i) * 16;
-      if (part == nullptr) {
-        Epilogue<T, EPI, BS>::run(g, piece, id.prob, m, n0 + (wn * G + j) * (GATED ? 32 : 64), lane);
-      } else if (m < g.M) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) part[((j * MT + i) * 4 + t) * 64] = piece[t];
-      }
+      for (int t = 0; t < 4; ++t) part[(p * 4 + t) * 64] = piece[t];
     }
+    __builtin_amdgcn_sched_barrier(0);  // pieces one after another: registers
+  }
 }
 
 // The tiles split over K: their slices' sums added in order, then as in k_dense.  One
 // wave per 16 m x 64 n (gated: 32 of each matrix) of a tile.
-template <typename T, int WM, int WN, int MT, int G, bool BS, int EPI>
+template <typename T, int WM, int WN, int MT, bool BS, int EPI>
 __global__ __launch_bounds__(256) void k_dense_join(GemmArgs g) {
   constexpr bool GATED = EPI == kGated || EPI == kGatedMax;
-  constexpr int NW = WM * WN, PIECES = NW * G * MT;
+  constexpr int NW = WM * WN, PIECES = NW * MT;
   typedef typename Mma<T>::Acc Acc;
   const int lane = threadIdx.x & 63;
   const int64_t piece = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int tail = (int)(piece / PIECES), rest = (int)(piece % PIECES);
-  const int wave = rest / (G * MT), j = rest / MT % G, i = rest % MT;
+  const int wave = rest / MT, i = rest % MT;
   if (tail >= g.tiles - g.whole) return;
   const TileId id = tile_at(g, g.whole + tail);
   const int m0 = id.m * (WM * MT * 16) + (wave / WN * MT + i) * 16;
   if (m0 >= g.M) return;
-  const int n0 = (id.n * WN * G + wave % WN * G + j) * (GATED ? 32 : 64);
-  const Acc* p = (const Acc*)g.part + ((int64_t)tail * g.slices * NW + wave) * (G * MT * 4 * 64) +
-                 (j * MT + i) * 4 * 64 + lane;
+  const int n0 = (id.n * WN + wave % WN) * (GATED ? 32 : 64);
+  const Acc* p = (const Acc*)g.part + ((int64_t)tail * g.slices * NW + wave) * (MT * 4 * 64) +
+                 i * 4 * 64 + lane;
+  typedef Epilogue<T, EPI, BS> E;
+  const typename E::In in = E::load(g, m0, n0, lane);
   Acc acc[4] = {};
-  for (int s = 0; s < g.slices; ++s)
+  constexpr int U = 8;  // slices in flight
+  for (int s = 0; s < g.slices; s += U) {
+    Acc v[U][4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[t] += p[(int64_t)s * NW * (G * MT * 4 * 64) + t * 64];
-  Epilogue<T, EPI, BS>::run(g, acc, id.prob, m0, n0, lane);
+    for (int j = 0; j < U; ++j)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        v[j][t] = s + j < g.slices ? p[(int64_t)(s + j) * NW * (MT * 4 * 64) + t * 64] : Acc{};
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (s + j < g.slices) acc[t] += v[j][t];
+  }
+  E::run(g, acc, in, id.prob, m0, n0, lane);
 }
 
 // ---- few rows of m ---------------------------------------------------------
@@ -669,7 +711,7 @@ __device__ __forceinline__ void join_waves(const GemmArgs& g, typename Mma<T>::A
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const int n = n0 + i * 16 + q * 4;
-      if (m < g.M && n < g.N) Epilogue<T, EPI, true>::tile(g, acc[i], 0, m, n);
+      Epilogue<T, EPI, true>::tile(g, acc[i], 0, m, n);
     }
   } else {
     Acc up = acc[S - 1];
@@ -691,7 +733,11 @@ __device__ __forceinline__ void join_waves(const GemmArgs& g, typename Mma<T>::A
       }
       Epilogue<T, EPI, true>::template gated<4>(g, gg, uu, m, n);
     } else {
-      unsigned mx = mine ? Epilogue<T, EPI, true>::scaled_gate(g, acc[0], up, m, n) : 0;
+      typedef Epilogue<T, EPI, true> E;
+      unsigned mx = 0;
+      if (mine)
+        mx = E::scaled_gate(g, acc[0], up, m, n, g.row_scale[m], E::cols4(g.col_scale[0], n, g.N),
+                            E::cols4(g.col_scale[1], n, g.N));
       mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
       mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
       if (q == 0 && m < g.M) atomicMax(g.row_max + m, mx);
@@ -833,14 +879,16 @@ __global__ __launch_bounds__(512) void k_dense_any(GemmArgs g) {
 }
 
 // ---- launching --------------------------------------------------------------
-template <typename T, int WM, int WN, int MT, int G, int SLOTS, bool AS, bool BS, int EPI>
+template <typename T, int WM, int WN, int MT, int SLOTS, bool AS, bool BS, int EPI>
 hipError_t launch_tile(const GemmArgs& g, hipStream_t s) {
   const int tail = g.tiles - g.whole;
   const int64_t blocks = g.whole + (int64_t)tail * g.slices;
-  k_dense<T, WM, WN, MT, G, SLOTS, AS, BS, EPI><<<(unsigned)blocks, WM * WN * 64, 0, s>>>(g);
+  constexpr size_t kLds = SLOTS * (WM * MT + WN * 4) * 16 * kStepBytes;
+  k_dense<T, WM, WN, MT, SLOTS, AS, BS, EPI>
+      <<<(unsigned)blocks, WM * WN * 64, kLds, s>>>(g);
   if (tail > 0) {
-    const int64_t waves = (int64_t)tail * WM * WN * G * MT;
-    k_dense_join<T, WM, WN, MT, G, BS, EPI><<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(g);
+    const int64_t waves = (int64_t)tail * WM * WN * MT;
+    k_dense_join<T, WM, WN, MT, BS, EPI><<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(g);
   }
   return hipGetLastError();
 }
@@ -866,11 +914,9 @@ hipError_t launch_shape(const GemmArgs& g, int shape, hipStream_t s) {
     case kRowsAny:
       if constexpr (!AS && !BS && EPI != kGateGrad) return launch_rows<T, EPI>(g, shape, s);
       return hipErrorInvalidValue;
-    case kTile256:  // fp32 is bound by its products, not by the LDS: smaller wave tiles
-      if constexpr (sizeof(T) == 4) return launch_tile<T, 2, 4, 8, 1, 2, AS, BS, EPI>(g, s);
-      else return launch_tile<T, 2, 2, 8, 2, 2, AS, BS, EPI>(g, s);
-    case kTile128: return launch_tile<T, 2, 2, 4, 1, 2, AS, BS, EPI>(g, s);
-    default: return launch_tile<T, 2, 2, 4, 1, 3, AS, BS, EPI>(g, s);
+    case kTile256: return launch_tile<T, 2, 4, 8, 2, AS, BS, EPI>(g, s);
+    case kTile128: return launch_tile<T, 2, 2, 4, 2, AS, BS, EPI>(g, s);
+    default: return launch_tile<T, 2, 2, 4, 3, AS, BS, EPI>(g, s);
   }
 }
 
