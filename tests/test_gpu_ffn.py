@@ -86,3 +86,20 @@ def test_gated_ffn_int8(cuda, T, h, I, dtype):
     qw = [t for m in w for t in F.quantize_int8(m)]
     want, bound = O.ffn_int8(x, *qw, dtype)
     O.assert_within(F.gated_ffn_int8(x, *qw), want, bound, "y")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("need", [(1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (0, 1, 0, 1),
+                                  (1, 0, 1, 0)])
+def test_some_gradients_only(cuda, need, dtype):
+    """What is not needed is not computed and changes nothing of the rest (within
+    the bounds: products are split as their own sizes ask)."""
+    args = layer(700, 264, 520, dtype, cuda)
+    dy = tokens(9, 700, 264, dtype, cuda)
+    for t, n in zip(args, need):
+        t.requires_grad_(bool(n))
+    y = F.gated_ffn(*args)
+    got = torch.autograd.grad(y, [t for t, n in zip(args, need) if n], dy)
+    ref = O.ffn_grads(*(t.detach() for t in args), dy)
+    for g, (w, b) in zip(got, [r for r, n in zip(ref, need) if n]):
+        O.assert_within(g, w, b, str(need))

@@ -255,11 +255,14 @@ struct Plan {
   size_t part_bytes;
 };
 
-float rounds_us(const ShapeCost& c, int64_t blocks, int steps) {
+// epi: bytes that the epilogue reads and writes per element of the tile.  A CU moves about
+// 20 KB a us; two blocks on a CU hide half of it behind each other's products.
+float rounds_us(const ShapeCost& c, int64_t blocks, int steps, float epi) {
   const int64_t cap = (int64_t)kCUs * c.per_cu, rest = blocks % cap;
-  const float full = steps * c.step + c.fixed;
+  const float move = epi * c.bm * c.bn / 20e3f;
+  const float full = steps * c.step + c.fixed + move;
   return blocks / cap * full +
-         (rest == 0 ? 0.0f : rest <= kCUs ? steps * c.alone + c.fixed : full);
+         (rest == 0 ? 0.0f : rest <= kCUs ? steps * c.alone + c.fixed + move : full);
 }
 
 // Rows of m up to which a product of two K-contiguous operands goes to k_dense_rows.
@@ -274,9 +277,10 @@ Plan plan_rows(int N, int K, int es, bool gated, bool any) {
   return {any ? kRowsAny : wide ? kRows32 : kRows16, waves, 1, blocks, blocks, blocks, 0};
 }
 
-// M x N x K per problem; gated: N columns of each of two matrices; rows: the few-row
-// kernels, any: for rows of any length.
-Plan plan_of(int M, int N, int K, int es, int nseg, int nprob, bool gated, bool rows, bool any) {
+// M x N x K per problem; gated: N columns of each of two matrices; epi: see rounds_us;
+// rows: the few-row kernels, any: for rows of any length.
+Plan plan_of(int M, int N, int K, int es, int nseg, int nprob, bool gated, float epi, bool rows,
+             bool any) {
   const int kb = 128 / es;
   const int steps = (K + kb - 1) / kb * nseg;
   if (rows) return plan_rows(N, K, es, gated, any);
@@ -293,9 +297,9 @@ Plan plan_of(int M, int N, int K, int es, int nseg, int nprob, bool gated, bool 
       if (S > 1 && (rest == 0 || part > kMaxPartBytes)) break;
       // Sums of rows past M are neither written nor read.
       const float moved = 2.0f * part * std::min(1.0f, (float)M / (tm * c.bm));
-      const float us = rounds_us(c, whole, steps) +
+      const float us = rounds_us(c, whole, steps, epi) +
                        (S == 1 ? 0.0f
-                               : rounds_us(c, rest * S, (steps + S - 1) / S) + 4.0f + moved / 4e6f);
+                               : rounds_us(c, rest * S, (steps + S - 1) / S, 4.0f) + 4.0f + moved / 4e6f);
       if (best.tiles == 0 || us < best_us) {
         best = {shape, S, (int)tm, (int)tn, (int)tiles, (int)whole, (size_t)part};
         best_us = us;
@@ -354,7 +358,13 @@ struct Call {
     const bool rows = g.M <= kRowsMax && form != kFormGateGrad && form != kFormKcKs &&
                       form != kFormKsKs;
     const bool any = g.lda % 16 != 0 || g.ldb % 16 != 0;
-    const Plan pl = plan_of(g.M, g.N, g.K, es(), g.nseg, g.nprob, gated, rows, any);
+    const int out = int8 ? 4 : es();  // int8: whatever the output's type, as the workspace
+    const float epi = form == kFormGateGrad    ? 8.0f + 2 * out
+                      : form == kFormGatedMax  ? 2.0f
+                      : form != kFormGated     ? out
+                      : g.out[1] != nullptr    ? out / 2 + 4
+                                               : out / 2;
+    const Plan pl = plan_of(g.M, g.N, g.K, es(), g.nseg, g.nprob, gated, epi, rows, any);
     reserve_part(pl);
     if (!go()) return;
     g.slices = pl.slices;
@@ -563,12 +573,20 @@ size_t wr_ffn_workspace_bytes(int backward, int dtype, int h, int I, int T) {
   a.intermediate_dim = I;
   a.batch_size = T;
   if (check_ffn(&a) != WR_OK) return 0;
-  return workspace_of(dtype, false, [&](Call& c) {
-    if (backward)
-      run_backward(c, a, true, true, true, true);
-    else
-      run_forward(c, a);
-  });
+  // The most that any call of these sizes takes: tiles and slices are chosen for what is
+  // kept (forward; the pointers are only compared) and needed (backward: one weight
+  // gradient alone has fewer tiles to share, and may be split more).
+  size_t most = 0;
+  for (const bool alone : {false, true}) {
+    if (alone) a.saved_gate = a.saved_up = reinterpret_cast<float*>(a.saved_act = &a);
+    most = std::max(most, workspace_of(dtype, false, [&](Call& c) {
+                      if (backward)
+                        run_backward(c, a, true, true, !alone, true);
+                      else
+                        run_forward(c, a);
+                    }));
+  }
+  return most;
 }
 
 int wr_ffn_forward(const wr_ffn_args* a, void* stream) {
