@@ -289,16 +289,19 @@ struct Epilogue {
   static __device__ __forceinline__ In load(const GemmArgs& g, int m0, int n0, int lane) {
     const int q = lane >> 4, m = m0 + (lane & 15);
     In in{};
-    if (m >= g.M) return in;
     if constexpr (EPI == kGateGrad) {
+      const int n = n0 + (lane & 15) * 4;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int n = col(n0, q, t);
-        if (n >= ((g.N + 7) & ~7)) continue;
-        in.v[t] = *(const f32x4*)((const float*)g.in[0] + (int64_t)m * g.ldi + n);
-        in.v[4 + t] = *(const f32x4*)((const float*)g.in[1] + (int64_t)m * g.ldi + n);
+      for (int j = 0; j < 4; ++j) {
+        const int row = m0 + j * 4 + q;
+        if (row >= g.M || n >= ((g.N + 7) & ~7)) continue;
+        in.v[j] = *(const f32x4*)((const float*)g.in[0] + (int64_t)row * g.ldi + n);
+        in.v[4 + j] = *(const f32x4*)((const float*)g.in[1] + (int64_t)row * g.ldi + n);
       }
-    } else if constexpr (EPI == kScale) {
+      return in;
+    }
+    if (m >= g.M) return in;
+    if constexpr (EPI == kScale) {
       in.row = g.row_scale[m];
 #pragma unroll
       for (int t = 0; t < 4; ++t) in.v[t] = cols4(g.col_scale[0], col(n0, q, t), g.N);
@@ -311,11 +314,34 @@ struct Epilogue {
     return in;
   }
 
-  // 16 m from m0, and 64 n from n0 (gated: 32 of gate, 32 of up) in 4 subtiles.
+  // 16 m from m0, and 64 n from n0 (gated: 32 of gate, 32 of up) in 4 subtiles.  lds: 4 KB of the
+  // wave's own.
   static __device__ __forceinline__ void run(const GemmArgs& g, const Acc (&acc)[4], const In& in,
-                                             int prob, int m0, int n0, int lane) {
-    const int q = lane >> 4, m = m0 + (lane & 15);
-    if constexpr (EPI == kGatedMax) {
+                                             int prob, int m0, int n0, int lane, char* lds) {
+    const int r = lane & 15, q = lane >> 4, m = m0 + r;
+    if constexpr (EPI == kGateGrad) {
+      // g, u, dg and du are 12 bytes per element of the tile, so that their lines count: the
+      // sums change lanes in LDS, and each access covers whole rows of the piece (256
+      // bytes of 4 rows) instead of 64 bytes of 16.
+#pragma unroll
+      for (int t = 0; t < 4; ++t) *(f32x4*)(lds + r * 256 + ((t * 4 + q) ^ r) * 16) = acc[t];
+      __builtin_amdgcn_wave_barrier();
+      const int n = n0 + r * 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = j * 4 + q;
+        const f32x4 da = *(const f32x4*)(lds + row * 256 + (r ^ row) * 16);
+        // dg and du rows are read in whole 16-byte chunks: their zeros past N too.
+        if (m0 + row >= g.M || n >= ((g.N + 7) & ~7)) continue;
+        float dg[4], du[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) gate_grad(da[i], in.v[j][i], in.v[4 + j][i], dg[i], du[i]);
+        const int64_t at = (int64_t)(m0 + row) * g.ldi + n;
+        store_run<T, 4>((T*)g.out[0] + at, dg, 4, true);
+        store_run<T, 4>((T*)g.out[1] + at, du, 4, true);
+      }
+      __builtin_amdgcn_wave_barrier();
+    } else if constexpr (EPI == kGatedMax) {
       gated_max(g, acc, in, m, n0 + q * 8);
     } else if (m >= g.M) {
       return;
@@ -337,22 +363,7 @@ struct Epilogue {
       store<16>(g, prob, m, n0 + q * 16, v);
     } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int n = col(n0, q, t);
-        if constexpr (EPI == kGateGrad) {
-          // dg and du rows are read in whole 16-byte chunks: their zeros past N too.
-          if (n >= ((g.N + 7) & ~7)) continue;
-          const int64_t at = (int64_t)m * g.ldi + n;
-          float dg[4], du[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            gate_grad(acc[t][i], in.v[t][i], in.v[4 + t][i], dg[i], du[i]);
-          store_run<T, 4>((T*)g.out[0] + at, dg, 4, true);
-          store_run<T, 4>((T*)g.out[1] + at, du, 4, true);
-        } else {
-          tile(g, acc[t], prob, m, n);
-        }
-      }
+      for (int t = 0; t < 4; ++t) tile(g, acc[t], prob, m, col(n0, q, t));
     }
   }
 
@@ -629,7 +640,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_dense(GemmArgs g) {
     if (part == nullptr) {
       typename E::In next{};
       if (p + 1 < MT) next = E::load(g, pm(p + 1), pn, lane);
-      E::run(g, piece, in, id.prob, pm(p), pn, lane);
+      E::run(g, piece, in, id.prob, pm(p), pn, lane, smem + wave * 4096);
       in = next;
     } else if (pm(p) < g.M) {
 #pragma unroll
@@ -674,7 +685,8 @@ __global__ __launch_bounds__(256) void k_dense_join(GemmArgs g) {
       for (int t = 0; t < 4; ++t)
         if (s + j < g.slices) acc[t] += v[j][t];
   }
-  E::run(g, acc, in, id.prob, m0, n0, lane);
+  __shared__ __attribute__((aligned(16))) char lds[4 * 4096];
+  E::run(g, acc, in, id.prob, m0, n0, lane, lds + (threadIdx.x >> 6) * 4096);
 }
 
 // ---- few rows of m ---------------------------------------------------------
