@@ -39,6 +39,7 @@ __global__ __launch_bounds__(256) void k_pad_rows(Pads pads) {
   const auto& job = pads.m[blockIdx.y];
   constexpr int N = 16 / sizeof(U);
   typedef U V __attribute__((ext_vector_type(N)));
+  typedef V V_any __attribute__((aligned(sizeof(U))));
   const int per = (int)(job.ld / 16);
   // Four rows a block in turn, a wave each.
   for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < job.rows;
@@ -46,9 +47,14 @@ __global__ __launch_bounds__(256) void k_pad_rows(Pads pads) {
     const U* const src = (const U*)job.src + row * job.cols;
     for (int i = threadIdx.x & 63; i < per; i += 64) {
       const int c = i * N;
-      V v;
+      V v{};
+      if (c + N <= job.cols) {
+        v = *(const V_any*)(src + c);
+      } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = c + j < job.cols ? src[c + j] : (U)0;
+        for (int j = 0; j < N; ++j)
+          if (c + j < job.cols) v[j] = src[c + j];
+      }
       *(V*)(job.dst + row * job.ld + i * 16) = v;
     }
   }
@@ -66,17 +72,16 @@ __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(f16 v) { return (float)v; }
 __device__ __forceinline__ float as_float(__bf16 v) { return (float)v; }
 
-// 127 x / m rounded to the nearest integer, ties to even, as the exact quotient
-// rounds.  In fp32 the quotient is off by less than 127 * 2^-22; where that could
-// reach a half-integer, or 127 x leaves the range, it is taken in 64 bits, whose
-// error (127 * 2^-53) is below the 2^-34 by which a quotient of two 24-bit
-// numbers misses a half-integer that it does not equal.
-__device__ __forceinline__ int code_of(float x, float m) {
-  const float t = x * 127.0f / m;
-  const float f = fabsf(t - rintf(t));
-  if (f > 0.4999f || !(m < 1e36f) || m < 1e-30f)
-    return (int)rint((double)x * 127.0 / (double)m);
-  return (int)rintf(t);
+// 127 x / m rounded to the nearest integer, ties to even, as the exact quotient rounds.
+// x times inv = 127 / m in fp32 is off by less than 127 * 2^-22; where that could reach a
+// half-integer, or inv leaves the range, the quotient is taken in 64 bits, whose error
+// (127 * 2^-53) is below the 2^-34 by which a quotient of two 24-bit numbers misses a
+// half-integer that it does not equal.  (A division per element took 20 us where the
+// product takes 15, 4096 x 4096 bf16: the vector instructions bound it.)
+__device__ __forceinline__ int code_of(float x, float m, float inv) {
+  const float t = x * inv, near = rintf(t);
+  if (fabsf(t - near) > 0.4999f || m < 1e-30f) return (int)rint((double)x * 127.0 / (double)m);
+  return (int)near;
 }
 
 // The scale of a row with maximum m (as fp32 bits).
@@ -84,13 +89,13 @@ __device__ __forceinline__ float scale_of(unsigned mx) {
   return mx >= 0x7f800000u ? __builtin_nanf("") : mx == 0 ? 1.0f : __uint_as_float(mx) / 127.0f;
 }
 
-constexpr int kQuantHeld = 4;  // vectors of a row that a thread keeps from the maximum to the codes
+constexpr int kQuantHeld = 2;  // vectors of a row that a thread keeps from the maximum to the codes
 
 // One block per row: max |row|, then the codes; a row's first kQuantHeld vectors per thread
 // stay in registers, what is longer is read again.  codes rows are ldc bytes apart, zero
-// from cols on.  zero_max, when set, gets its word of the row cleared.  VEC: rows are
-// whole 16-byte vectors.
-template <typename T, bool VEC>
+// from cols on.  zero_max, when set, gets its word of the row cleared.  WHOLE: cols is a
+// multiple of a vector.
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(1024) void k_quantize(const T* __restrict__ x, int cols,
                                                    int8_t* __restrict__ codes, int64_t ldc,
                                                    float* __restrict__ scales,
@@ -98,10 +103,23 @@ __global__ __launch_bounds__(1024) void k_quantize(const T* __restrict__ x, int 
   __shared__ unsigned part[16];
   const int64_t row = blockIdx.x;
   const T* p = x + row * cols;
-  constexpr int N = VEC ? 16 / sizeof(T) : 1;
+  constexpr int N = 16 / sizeof(T);
   typedef T V __attribute__((ext_vector_type(N)));
+  typedef V V_any __attribute__((aligned(sizeof(T))));
   typedef int8_t Q __attribute__((ext_vector_type(N)));
+  typedef Q Q_any __attribute__((aligned(1)));
   const int step = blockDim.x * N;
+  auto read = [&](int c) {  // the vector at column c, zero from cols on
+    V v{};
+    if (WHOLE ? c < cols : c + N <= cols) {
+      v = *(const V_any*)(p + c);
+    } else if (!WHOLE) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c + i < cols) v[i] = p[c + i];
+    }
+    return v;
+  };
   auto top = [](V v) {
     unsigned mx = 0;
 #pragma unroll
@@ -111,15 +129,10 @@ __global__ __launch_bounds__(1024) void k_quantize(const T* __restrict__ x, int 
   V held[kQuantHeld];
   unsigned mx = 0;
 #pragma unroll
-  for (int j = 0; j < kQuantHeld; ++j) {
-    const int c = threadIdx.x * N + j * step;
-    held[j] = V{};
-    if (c < cols) held[j] = *(const V*)(p + c);
-  }
+  for (int j = 0; j < kQuantHeld; ++j) held[j] = read(threadIdx.x * N + j * step);
 #pragma unroll
   for (int j = 0; j < kQuantHeld; ++j) mx = max(mx, top(held[j]));
-  for (int c = threadIdx.x * N + kQuantHeld * step; c < cols; c += step)
-    mx = max(mx, top(*(const V*)(p + c)));
+  for (int c = threadIdx.x * N + kQuantHeld * step; c < cols; c += step) mx = max(mx, top(read(c)));
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) mx = max(mx, (unsigned)__shfl_xor((int)mx, d));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
@@ -130,20 +143,26 @@ __global__ __launch_bounds__(1024) void k_quantize(const T* __restrict__ x, int 
     if (zero_max != nullptr) zero_max[row] = 0;
   }
   const bool live = mx < 0x7f800000u && mx != 0;
-  const float m = __uint_as_float(mx);
+  const float m = __uint_as_float(mx), inv = 127.0f / m;
   int8_t* const q = codes + row * ldc;
   auto code = [&](int c, V v) {
-    Q o;
+    if (c >= cols) return;
+    Q o{};
+    if (live) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = live ? (int8_t)code_of(as_float(v[i]), m) : (int8_t)0;
-    *(Q*)(q + c) = o;
+      for (int i = 0; i < N; ++i) o[i] = (int8_t)code_of(as_float(v[i]), m, inv);
+    }
+    if (WHOLE || c + N <= cols) {
+      *(Q_any*)(q + c) = o;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c + i < cols) q[c + i] = o[i];
+    }
   };
 #pragma unroll
-  for (int j = 0; j < kQuantHeld; ++j) {
-    const int c = threadIdx.x * N + j * step;
-    if (c < cols) code(c, held[j]);
-  }
-  for (int c = threadIdx.x * N + kQuantHeld * step; c < cols; c += step) code(c, *(const V*)(p + c));
+  for (int j = 0; j < kQuantHeld; ++j) code(threadIdx.x * N + j * step, held[j]);
+  for (int c = threadIdx.x * N + kQuantHeld * step; c < cols; c += step) code(c, read(c));
   for (int c = cols + threadIdx.x; c < (int)ldc; c += blockDim.x) q[c] = 0;
 }
 
@@ -163,9 +182,10 @@ __global__ __launch_bounds__(256) void k_quantize_known(const float* __restrict_
     Q o{};
     if (mx < 0x7f800000u && mx != 0 && c < cols) {
       const f32x4 v = *(const f32x4*)(x + row * ldx + c);
+      const float m = __uint_as_float(mx), inv = 127.0f / m;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (c + i < cols) o[i] = (int8_t)code_of(v[i], __uint_as_float(mx));
+        if (c + i < cols) o[i] = (int8_t)code_of(v[i], m, inv);
     }
     *(Q*)(codes + row * ldx + c) = o;
   }
@@ -174,12 +194,10 @@ __global__ __launch_bounds__(256) void k_quantize_known(const float* __restrict_
 template <typename T>
 hipError_t launch_quantize_as(const T* x, int rows, int cols, int8_t* codes, int64_t ldc,
                               float* scales, unsigned* zero_max, hipStream_t s) {
-  constexpr int N = 16 / sizeof(T);
   // Two vectors a thread: their latency overlaps, and short rows take few waves.
-  const bool vec = cols % N == 0;
-  const int per = 2 * (vec ? N : 1);
+  constexpr int per = 2 * 16 / sizeof(T);
   const int threads = std::min(1024, std::max(64, (cols + per * 64 - 1) / (per * 64) * 64));
-  if (vec)
+  if (cols % (per / 2) == 0)
     k_quantize<T, true><<<rows, threads, 0, s>>>(x, cols, codes, ldc, scales, zero_max);
   else
     k_quantize<T, false><<<rows, threads, 0, s>>>(x, cols, codes, ldc, scales, zero_max);
@@ -265,16 +283,17 @@ float rounds_us(const ShapeCost& c, int64_t blocks, int steps, float epi) {
          (rest == 0 ? 0.0f : rest <= kCUs ? steps * c.alone + c.fixed + move : full);
 }
 
-// Rows of m up to which a product of two K-contiguous operands goes to k_dense_rows.
-constexpr int kRowsMax = 16;
+// Rows of m up to which a product of two K-contiguous operands goes to k_dense_rows, and,
+// where a row is no whole 16-byte chunks, to k_dense_any.
+constexpr int kRowsMax = 16, kAnyMax = 64;
 // 32 rows of B a block where that leaves 2 blocks a CU, else 16; 8 waves a block
 // where there are fewer blocks than CUs, else 4.
-Plan plan_rows(int N, int K, int es, bool gated, bool any) {
+Plan plan_rows(int M, int N, int K, int es, bool gated, bool any) {
   const int64_t steps = ((int64_t)K * es + 127) / 128;
   const bool wide = !any && (N + (gated ? 15 : 31)) / (gated ? 16 : 32) >= 2 * kCUs;
   const int rows = (wide ? 32 : 16) / (gated ? 2 : 1), blocks = (N + rows - 1) / rows;
-  const int waves = blocks < kCUs && steps >= 16 ? 8 : 4;
-  return {any ? kRowsAny : wide ? kRows32 : kRows16, waves, 1, blocks, blocks, blocks, 0};
+  const int tm = (M + 15) / 16, waves = blocks * tm < kCUs && steps >= 16 ? 8 : 4;
+  return {any ? kRowsAny : wide ? kRows32 : kRows16, waves, tm, blocks, blocks * tm, blocks * tm, 0};
 }
 
 // M x N x K per problem; gated: N columns of each of two matrices; epi: see rounds_us;
@@ -283,7 +302,7 @@ Plan plan_of(int M, int N, int K, int es, int nseg, int nprob, bool gated, float
              bool any) {
   const int kb = 128 / es;
   const int steps = (K + kb - 1) / kb * nseg;
-  if (rows) return plan_rows(N, K, es, gated, any);
+  if (rows) return plan_rows(M, N, K, es, gated, any);
   Plan best{};
   float best_us = 0;
   for (int shape = 0; shape < kShapes; ++shape) {
@@ -355,9 +374,9 @@ struct Call {
   void product(GemmArgs g, int form) {
     const bool gated = form == kFormGated || form == kFormGatedMax;
     if (g.M == 0 || g.N == 0) return;
-    const bool rows = g.M <= kRowsMax && form != kFormGateGrad && form != kFormKcKs &&
-                      form != kFormKsKs;
     const bool any = g.lda % 16 != 0 || g.ldb % 16 != 0;
+    const bool rows = (any || g.M <= kRowsMax) && form != kFormGateGrad && form != kFormKcKs &&
+                      form != kFormKsKs;
     const int out = int8 ? 4 : es();  // int8: whatever the output's type, as the workspace
     const float epi = form == kFormGateGrad    ? 8.0f + 2 * out
                       : form == kFormGatedMax  ? 2.0f
@@ -373,8 +392,6 @@ struct Call {
     g.tiles = pl.tiles;
     g.whole = pl.whole;
     g.part = ws + part_at;
-    const int oes = int8 ? elem_bytes(g.out_dtype) : es();
-    g.vec = g.ldo * oes % 16 == 0;
     check(int8 ? launch_i8(g, pl.shape, form, stream)
           : dtype == WR_F32 ? launch_f32(g, pl.shape, form, stream)
           : dtype == WR_F16 ? launch_f16(g, pl.shape, form, stream)
@@ -399,7 +416,7 @@ void run_forward(Call& c, const wr_ffn_args& a) {
   const int T = a.batch_size, h = a.hidden_dim, I = a.intermediate_dim;
   const int64_t Ip = round_up(I, 64);
   const bool keep = a.saved_act != nullptr;
-  const bool few = T <= kRowsMax;
+  const bool few = T <= kAnyMax;
   const Call::Mat x = c.rows16(a.x, T, h, few);
   const Call::Mat wg = c.rows16(a.w_gate, I, h, few), wu = c.rows16(a.w_up, I, h, few);
   const Call::Mat wd = c.rows16(a.w_down, h, I, few);
@@ -471,7 +488,7 @@ void run_backward(Call& c, const wr_ffn_args& a, bool dx, bool dwg, bool dwu, bo
 }
 
 void run_int8(Call& c, const wr_int8_args& a) {
-  const bool few = a.rows <= kRowsMax;
+  const bool few = a.rows <= kAnyMax;
   const Call::Mat x = c.rows16(a.x, a.rows, a.in_features, few);
   const Call::Mat w = c.rows16(a.w, a.out_features, a.in_features, few);
   c.pad();
@@ -493,7 +510,7 @@ void run_ffn_int8(Call& c, const wr_ffn_int8_args& a) {
   float* act = (float*)c.take(T * Ip * 4);
   int8_t* aq = (int8_t*)c.take(T * Ip);
   float* sa = (float*)c.take((int64_t)T * 4);
-  const bool few = T <= kRowsMax;
+  const bool few = T <= kAnyMax;
   const Call::Mat wg = c.rows16(a.w_gate, I, h, few), wu = c.rows16(a.w_up, I, h, few);
   const Call::Mat wd = c.rows16(a.w_down, h, I, few);
   c.pad();

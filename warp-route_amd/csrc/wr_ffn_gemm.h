@@ -235,16 +235,17 @@ __device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-
 // g * sigmoid(g)
 __device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
 
-// N consecutive elements at p[0..N), of which the first `left` exist.  VEC: p is
-// aligned to its N elements.
+// N consecutive elements at p[0..N), of which the first `left` exist.  p has its element's
+// alignment: a store that is not aligned to its size is still one instruction.
 template <typename T, int N>
-__device__ __forceinline__ void store_run(T* p, const float* v, int left, bool vec) {
-  if (vec && left >= N) {
+__device__ __forceinline__ void store_run(T* p, const float* v, int left) {
+  if (left >= N) {
     typedef T V __attribute__((ext_vector_type(N)));
+    typedef V V_any __attribute__((aligned(sizeof(T))));
     V o;
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = to_out<T>(v[i]);
-    *(V*)p = o;
+    *(V_any*)p = o;
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -337,8 +338,8 @@ struct Epilogue {
 #pragma unroll
         for (int i = 0; i < 4; ++i) gate_grad(da[i], in.v[j][i], in.v[4 + j][i], dg[i], du[i]);
         const int64_t at = (int64_t)(m0 + row) * g.ldi + n;
-        store_run<T, 4>((T*)g.out[0] + at, dg, 4, true);
-        store_run<T, 4>((T*)g.out[1] + at, du, 4, true);
+        store_run<T, 4>((T*)g.out[0] + at, dg, 4);
+        store_run<T, 4>((T*)g.out[1] + at, du, 4);
       }
       __builtin_amdgcn_wave_barrier();
     } else if constexpr (EPI == kGatedMax) {
@@ -374,7 +375,7 @@ struct Epilogue {
     O* const p = (O*)g.out[prob] + (int64_t)m * g.ldo + n;
     constexpr int V = 16 / sizeof(O) < C ? 16 / sizeof(O) : C;
 #pragma unroll
-    for (int i = 0; i < C; i += V) store_run<O, V>(p + i, v + i, g.N - n - i, g.vec);
+    for (int i = 0; i < C; i += V) store_run<O, V>(p + i, v + i, g.N - n - i);
   }
   template <int C>
   static __device__ __forceinline__ void store(const GemmArgs& g, int prob, int m, int n,
@@ -410,12 +411,12 @@ struct Epilogue {
     const int64_t at = (int64_t)m * g.ldi + n;
     constexpr int V = 16 / sizeof(T) < C ? 16 / sizeof(T) : C;
 #pragma unroll
-    for (int i = 0; i < C; i += V) store_run<T, V>((T*)g.out[0] + at + i, a + i, V, true);
+    for (int i = 0; i < C; i += V) store_run<T, V>((T*)g.out[0] + at + i, a + i, V);
     if (g.out[1] != nullptr) {
 #pragma unroll
       for (int i = 0; i < C; i += 4) {
-        store_run<float, 4>((float*)g.out[1] + at + i, gg + i, 4, true);
-        store_run<float, 4>((float*)g.out[2] + at + i, uu + i, 4, true);
+        store_run<float, 4>((float*)g.out[1] + at + i, gg + i, 4);
+        store_run<float, 4>((float*)g.out[2] + at + i, uu + i, 4);
       }
     }
   }
@@ -445,7 +446,7 @@ struct Epilogue {
       if (n + i >= g.N) v[i] = 0.0f;  // a NaN row scale times the zero
       mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
     }
-    store_run<float, 4>((float*)g.out[0] + (int64_t)m * g.ldi + n, v, 4, true);
+    store_run<float, 4>((float*)g.out[0] + (int64_t)m * g.ldi + n, v, 4);
     return mx;
   }
 };
@@ -705,7 +706,8 @@ constexpr int kRowSlots = 3;
 // Joins the waves' sums (acc[S] of each) in LDS and runs the epilogue.
 template <typename T, int S, int EPI>
 __device__ __forceinline__ void join_waves(const GemmArgs& g, typename Mma<T>::Acc (&acc)[S],
-                                           char* lds, int n0, int wave, int waves, int lane) {
+                                           char* lds, int m0, int n0, int wave, int waves,
+                                           int lane) {
   constexpr bool GATED = EPI == kGated || EPI == kGatedMax;
   typedef typename Mma<T>::Acc Acc;
   const int r = lane & 15, q = lane >> 4;
@@ -718,7 +720,7 @@ __device__ __forceinline__ void join_waves(const GemmArgs& g, typename Mma<T>::A
 #pragma unroll
   for (int i = 0; i < S; ++i)
     for (int w = 1; w < waves; ++w) acc[i] += sums[(w * S + i) * 64 + lane];
-  const int m = r;
+  const int m = m0 + r;
   if constexpr (!GATED) {
 #pragma unroll
     for (int i = 0; i < S; ++i) {
@@ -824,11 +826,12 @@ __global__ __launch_bounds__(512) void k_dense_rows(GemmArgs g) {
     fill = fill + 1 == kRowSlots ? 0 : fill + 1;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  join_waves<T, S, EPI>(g, acc, smem, n0, wave, waves, lane);
+  join_waves<T, S, EPI>(g, acc, smem, 0, n0, wave, waves, lane);
 }
 
-// k_dense_any: the same for rows that are no whole 16-byte chunks, with loads straight
-// into the products' registers: 16 bytes of one row a lane, of any alignment.  Rows past
+// k_dense_any: up to 64 rows of m, for rows that are no whole 16-byte chunks (which the tiled
+// products need copied first), with loads straight into the products' registers: 16
+// bytes of one row a lane, of any alignment.  Rows past
 // the matrices' ends read the last one again, their results are dropped.
 typedef u32x4 u32x4_any __attribute__((aligned(1)));
 
@@ -855,10 +858,14 @@ __global__ __launch_bounds__(512) void k_dense_any(GemmArgs g) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int n0 = blockIdx.x * (GATED ? 8 : 16);
+  // Blocks 8 apart run on one XCD: its L2 serves B's rows to all their tiles of m.
+  const int place = blockIdx.x >> 3;
+  const int m0 = place % g.tiles_m * 16;
+  const int n0 = (place / g.tiles_m * 8 + (blockIdx.x & 7)) * (GATED ? 8 : 16);
+  if (n0 >= g.N) return;
   const int row = min(n0 + (GATED ? r & 7 : r), g.N - 1);
   const char* const pb = g.b[GATED ? r >> 3 : 0] + row * g.ldb;
-  const char* const pa = g.a[0] + min(r, g.M - 1) * g.lda;
+  const char* const pa = g.a[0] + min(m0 + r, g.M - 1) * g.lda;
 
   // 64-byte stages of K in whole 128-byte pairs per wave.
   const int stages = (g.K + KB - 1) / KB, per = (stages + 2 * waves - 1) / (2 * waves) * 2;
@@ -887,7 +894,7 @@ __global__ __launch_bounds__(512) void k_dense_any(GemmArgs g) {
     const int k = s * KB + q * EPC;
     acc[0] = Mma<T>::add(load_tail<T>(pb, k, g.K), load_tail<T>(pa, k, g.K), acc[0]);
   }
-  join_waves<T, 1, EPI>(g, acc, smem, n0, wave, waves, lane);
+  join_waves<T, 1, EPI>(g, acc, smem, m0, n0, wave, waves, lane);
 }
 
 // ---- launching --------------------------------------------------------------
@@ -910,7 +917,7 @@ hipError_t launch_rows(const GemmArgs& g, int shape, hipStream_t s) {
   const unsigned blocks = (unsigned)g.tiles;
   const int waves = g.slices;
   if (shape == kRowsAny)
-    k_dense_any<T, EPI><<<blocks, waves * 64, waves * 1024, s>>>(g);
+    k_dense_any<T, EPI><<<(g.tiles_n + 7) / 8 * 8 * g.tiles_m, waves * 64, waves * 1024, s>>>(g);
   else if (shape == kRows16)
     k_dense_rows<T, 1, EPI><<<blocks, waves * 64, waves * kRowSlots * 4096, s>>>(g);
   else

@@ -34,7 +34,6 @@ struct GemmArgs {
   const float* col_scale[2];
   unsigned* row_max;
   int out_dtype;
-  bool vec;  // out rows and pointer are 16-byte aligned
 };
 
 // Tile shapes (m x n; gated products: n / 2 columns of each matrix): 256 x 256, 128 x 128,
