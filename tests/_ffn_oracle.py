@@ -120,7 +120,11 @@ def ffn_int8(x, wg, sg, wu, su, wd, sd, dtype):
     flip = ((t - torch.floor(t) - 0.5).abs() <= et).double()
     sa = safe / 127.0
     y = (qa @ wd.double().t()) * sa * sd.double()
-    e = (flip @ wd.double().abs().t()) * sa * sd.double() + y.abs() * (em / safe + 4 * E)
+    # The kernel's sum is (sum (qa + f) w) sa (1 + d) sd with codes off by f, |f| <= flip, and
+    # its scale and roundings off by |d| <= em / safe + 4 E: it differs from y by at most
+    # |sum f w| sa sd (1 + |d|) + |y| |d|.
+    d = em / safe + 4 * E
+    e = (flip @ wd.double().abs().t()) * sa * sd.double() * (1 + d) + y.abs() * d
     return y, e + u(dtype) * (y.abs() + e) + step(dtype)
 
 

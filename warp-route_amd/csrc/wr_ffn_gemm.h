@@ -336,7 +336,10 @@ struct Epilogue {
         if (m0 + row >= g.M || n >= ((g.N + 7) & ~7)) continue;
         float dg[4], du[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) gate_grad(da[i], in.v[j][i], in.v[4 + j][i], dg[i], du[i]);
+        for (int i = 0; i < 4; ++i) {
+          gate_grad(da[i], in.v[j][i], in.v[4 + j][i], dg[i], du[i]);
+          if (n + i >= g.N) dg[i] = du[i] = 0.0f;
+        }
         const int64_t at = (int64_t)(m0 + row) * g.ldi + n;
         store_run<T, 4>((T*)g.out[0] + at, dg, 4);
         store_run<T, 4>((T*)g.out[1] + at, du, 4);
@@ -400,14 +403,15 @@ struct Epilogue {
   }
 
   // C gate and up sums of the same n.  The buffers' rows are padded to ldi (a multiple of
-  // 64) and the sums past N are zero, so whole vectors are stored.
+  // 64), so whole vectors are stored; a is read in whole 16-byte chunks, so its values
+  // past N are zeros (the sums there are not, where x holds an infinity).
   template <int C>
   static __device__ __forceinline__ void gated(const GemmArgs& g, const float (&gg)[C],
                                                const float (&uu)[C], int m, int n) {
     if (n >= ((g.N + 7) & ~7)) return;
     float a[C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) a[i] = silu(gg[i]) * uu[i];
+    for (int i = 0; i < C; ++i) a[i] = n + i < g.N ? silu(gg[i]) * uu[i] : 0.0f;
     const int64_t at = (int64_t)m * g.ldi + n;
     constexpr int V = 16 / sizeof(T) < C ? 16 / sizeof(T) : C;
 #pragma unroll
@@ -742,8 +746,8 @@ __device__ __forceinline__ void join_waves(const GemmArgs& g, typename Mma<T>::A
       float gg[4], uu[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        gg[i] = n + i < g.N ? acc[0][i] : 0.0f;
-        uu[i] = n + i < g.N ? up[i] : 0.0f;
+        gg[i] = acc[0][i];
+        uu[i] = up[i];
       }
       Epilogue<T, EPI, true>::template gated<4>(g, gg, uu, m, n);
     } else {

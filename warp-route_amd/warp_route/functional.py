@@ -408,6 +408,34 @@ class _GatedFFN(torch.autograd.Function):
             dy.contiguous(), *ctx.saved_tensors, list(ctx.needs_input_grad)))
 
 
+_EAGER = "warp_route.eager_graph"  # metadata key of a leaf's gradient accumulator
+
+
+def _accumulators(tensors):
+    """Metadata of the leaves' gradient accumulators, which live as long as a
+    graph that uses them."""
+    for t in tensors:
+        if t.requires_grad and t.is_leaf:
+            yield torch.autograd.graph.get_gradient_edge(t).node.metadata
+
+
+def _differentiable_ffn(leaves, *args: torch.Tensor) -> torch.Tensor:
+    """_GatedFFN, refused under graph capture while an eager graph of the leaves
+    among ``leaves`` is alive.  Their gradient accumulators then belong to the eager
+    graph's stream, for which the captured backward pass would wait; torch does
+    not survive that.  Eager calls mark the accumulators, captured ones look
+    for the mark."""
+    if not args[0].is_cuda or not torch.cuda.is_current_stream_capturing():
+        y = _GatedFFN.apply(*args)
+        for mark in _accumulators(leaves):
+            mark[_EAGER] = True
+        return y
+    if any(_EAGER in mark for mark in _accumulators(leaves)):
+        raise RuntimeError("gated_ffn is captured into a graph while an eager autograd graph of "
+                           "the same tensors is alive: drop its outputs before the capture")
+    return _GatedFFN.apply(*args)
+
+
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x [..., n] as [rows, n]."""
     if x.dim() == 0:
@@ -433,12 +461,14 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     arguments; gradients that are not needed are not computed.
 
     Forward and backward launch kernels on the current stream only and may be
-    captured in a HIP graph.  As for any torch operator, no eager graph of the
-    same leaf tensors may be alive when a backward pass is captured.
+    captured in a HIP graph.  When a backward pass is captured, no eager graph
+    of the same leaf tensors may be alive (as for any torch operator); one
+    that a call of this function made raises RuntimeError.
     """
     rows = _rows(x)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
-        y = _GatedFFN.apply(rows, w_gate, w_up, w_down)
+    leaves = (x, w_gate, w_up, w_down)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in leaves):
+        y = _differentiable_ffn(leaves, rows, w_gate, w_up, w_down)
     else:
         y = _load_extension().gated_ffn_forward(rows, w_gate, w_up, w_down, False)[0]
     return y if x.dim() == 2 else y.reshape(x.shape)
@@ -462,6 +492,9 @@ def int8_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     token and per output channel (``quantize_int8``).  The sum is exact; it is
     scaled in fp32 and rounded once to out_dtype (float32, float16 or
     bfloat16)."""
+    if x_scale.shape != x.shape[:-1]:
+        raise ValueError(f"x_scale must have shape {tuple(x.shape[:-1])}, got "
+                         f"{tuple(x_scale.shape)}")
     out = _load_extension().int8_matmul(_rows(x), x_scale.reshape(-1), w, w_scale, out_dtype)
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], out.shape[-1])
 
