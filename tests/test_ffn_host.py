@@ -156,8 +156,10 @@ def test_python_entry_points_refuse_host_tensors():
                                        torch.ones(4))):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
-    with pytest.raises(ValueError, match="dimension"):
+    with pytest.raises(RuntimeError, match="dimension"):
         F.gated_ffn(torch.tensor(1.0), w, w, w)
+    with pytest.raises(ValueError, match="dimension"):
+        F.quantize_int8(torch.tensor(1.0))
     with pytest.raises(ValueError, match="x_scale"):
         F.int8_matmul(x.to(torch.int8), torch.ones(3), w.to(torch.int8), torch.ones(4))
 

@@ -322,6 +322,50 @@ def test_capture_beside_a_live_eager_graph_is_refused(cuda):
     assert all(torch.isfinite(g).all() for g in grads)
 
 
+def test_two_calls_of_the_same_weights(cuda):
+    """Weights used twice, eagerly and within one capture: gradients add up."""
+    x, *w = layer(6, 64, 96, torch.float32, cuda)
+    for t in w:
+        t.requires_grad_(True)
+
+    def step():
+        y = F.gated_ffn(F.gated_ffn(x, *w), *w)
+        return [y.detach(), *torch.autograd.grad(y, w, torch.ones_like(y))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(3):
+        eager = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, captured))
+    mid = F.gated_ffn(x, *(t.detach() for t in w))
+    inner = mid.clone().requires_grad_(True)
+    gin, *second = torch.autograd.grad(F.gated_ffn(inner, *w), [inner, *w], torch.ones_like(mid))
+    first = torch.autograd.grad(F.gated_ffn(x, *w), w, gin)
+    for a, b, c in zip(eager[1:], first, second):
+        assert torch.equal(a, b + c)
+
+
+def test_differentiable_once(cuda):
+    args = [t.requires_grad_(True) for t in layer(3, 32, 48, torch.float32, cuda)]
+    y = F.gated_ffn(*args)
+    grads = torch.autograd.grad(y, args, torch.ones_like(y), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        grads[0].sum().backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y = F.gated_ffn(*args)
+        with torch.no_grad():
+            args[1].mul_(2)
+        torch.autograd.grad(y, args, torch.ones_like(y))
+
+
 def test_rows_past_32_bit_offsets(cuda):
     """150000 x 16384 activations: 2.5e9 elements.  The last rows, which lie past
     2^32 bytes, are those of a call on these rows alone, and their own oracle."""

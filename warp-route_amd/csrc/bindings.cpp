@@ -24,8 +24,12 @@
 // *MasqueradingAsCUDA guard and stream accessors accept that device type.
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <hip/hip_runtime_api.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <array>
 #include <atomic>
 #include <cstdlib>
 #include <optional>
@@ -446,6 +450,86 @@ std::vector<std::optional<torch::Tensor>> gated_ffn_backward(
   return out;
 }
 
+// The differentiable form: y, with what the backward pass reads kept when a gradient is
+// needed.  Differentiable once: the gradients of a backward pass that builds a graph
+// raise when they are differentiated themselves.
+class GatedFfn : public torch::autograd::Function<GatedFfn> {
+ public:
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& x,
+                               const torch::Tensor& w_gate, const torch::Tensor& w_up,
+                               const torch::Tensor& w_down) {
+    std::vector<torch::Tensor> r = gated_ffn_forward(x, w_gate, w_up, w_down, true);
+    ctx->save_for_backward({x, w_gate, w_up, w_down, r[1], r[2], r[3]});
+    return r[0];
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const torch::autograd::variable_list s = ctx->get_saved_variables();
+    std::vector<bool> need(4);
+    for (int i = 0; i < 4; ++i) need[i] = ctx->needs_input_grad(i);
+    torch::autograd::variable_list out(4);
+    {
+      const at::AutoGradMode off(false);
+      const auto got = gated_ffn_backward(grads[0].contiguous(), s[0], s[1], s[2], s[3], s[4], s[5],
+                                          s[6], need);
+      for (int i = 0; i < 4; ++i)
+        if (got[i].has_value()) out[i] = *got[i];
+    }
+    if (at::GradMode::is_enabled()) {
+      auto once = std::make_shared<torch::autograd::DelayedError>(
+          "gated_ffn is differentiable once: its gradients cannot be differentiated", 1);
+      for (torch::Tensor& t : out) {
+        if (!t.defined()) continue;
+        t.set_requires_grad(true);
+        t = (*once)({t})[0];
+      }
+    }
+    return out;
+  }
+};
+
+// Under graph capture, gradient accumulators of leaves that an eager graph keeps alive
+// belong to that graph's stream.  A captured backward pass would wait for it, which
+// torch does not survive: refused here.
+void check_capture(const std::array<torch::Tensor, 4>& leaves, const torch::Device& dev) {
+  const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess ||
+      status == hipStreamCaptureStatusNone)
+    return;
+  for (const torch::Tensor& t : leaves) {
+    if (!t.requires_grad() || !t.is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto home = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!home.has_value() || *home == stream.unwrap(),
+                "gated_ffn is captured into a graph while an eager autograd graph of the same "
+                "tensors is alive: drop its outputs before the capture");
+  }
+}
+
+// gated_ffn(x [.., h], w_gate, w_up, w_down) -> y, differentiable where a gradient is asked for.
+torch::Tensor gated_ffn(const torch::Tensor& x, const torch::Tensor& w_gate,
+                        const torch::Tensor& w_up, const torch::Tensor& w_down) {
+  TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA (HIP) tensor");
+  TORCH_CHECK(x.is_contiguous(), "x must be contiguous");
+  const int64_t h = x.size(-1);
+  const torch::Tensor rows =
+      x.dim() == 2 ? x : x.reshape({h > 0 ? x.numel() / h : x.numel(), h});
+  torch::Tensor y;
+  const std::array<torch::Tensor, 4> leaves{x, w_gate, w_up, w_down};
+  bool grad = false;
+  for (const torch::Tensor& t : leaves) grad = grad || t.requires_grad();
+  if (grad && at::GradMode::is_enabled()) {
+    check_capture(leaves, x.device());
+    y = GatedFfn::apply(rows, w_gate, w_up, w_down);
+  } else {
+    y = gated_ffn_forward(rows, w_gate, w_up, w_down, false)[0];
+  }
+  return x.dim() == 2 ? y : y.reshape(x.sizes());
+}
+
 // quantize_int8(x [rows, cols]) -> (codes int8, scales fp32 [rows]).
 std::tuple<torch::Tensor, torch::Tensor> quantize_int8(torch::Tensor x) {
   check_tokens(x, "x");
@@ -583,6 +667,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gate_topk", &gate_topk, "Router logits, softmax and top-K", py::arg("hidden"),
         py::arg("gate_w"), py::arg("num_experts"), py::arg("hidden_dim"), py::arg("top_k"),
         py::arg("renormalize") = false);
+  m.def("gated_ffn", &gated_ffn, "Dense gated FFN (fp32, fp16 or bf16), differentiable",
+        py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("w_down"));
   m.def("gated_ffn_forward", &gated_ffn_forward,
         "Dense gated FFN (fp32, fp16 or bf16); with keep also what its backward pass reads",
         py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("w_down"),

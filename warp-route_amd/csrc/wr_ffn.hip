@@ -314,8 +314,8 @@ Plan plan_of(int M, int N, int K, int es, int nseg, int nprob, bool gated, float
       const int64_t whole = S == 1 ? tiles : tiles - rest;
       const int64_t part = (tiles - whole) * S * c.bm * c.bn * 4;
       if (S > 1 && (rest == 0 || part > kMaxPartBytes)) break;
-      // Sums of rows past M are neither written nor read.
-      const float moved = 2.0f * part * std::min(1.0f, (float)M / (tm * c.bm));
+      // The join reads them (they are written like an epilogue); not those of rows past M.
+      const float moved = part * std::min(1.0f, (float)M / (tm * c.bm));
       const float us = rounds_us(c, whole, steps, epi) +
                        (S == 1 ? 0.0f
                                : rounds_us(c, rest * S, (steps + S - 1) / S, 4.0f) + 4.0f + moved / 4e6f);

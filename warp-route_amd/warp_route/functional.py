@@ -390,52 +390,6 @@ def gate_topk(
     return _C.gate_topk(x, gate_w, num_experts, hidden_dim, top_k, renormalize)
 
 
-class _GatedFFN(torch.autograd.Function):
-    """gated_ffn with its backward pass.  Keeps g = x w_gate^T, u = x w_up^T and
-    silu(g) u (fp32, fp32 and x's dtype; rows padded to 64 elements) for the
-    gradients."""
-
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down):
-        y, g, u, a = _load_extension().gated_ffn_forward(x, w_gate, w_up, w_down, True)
-        ctx.save_for_backward(x, w_gate, w_up, w_down, g, u, a)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        return tuple(_load_extension().gated_ffn_backward(
-            dy.contiguous(), *ctx.saved_tensors, list(ctx.needs_input_grad)))
-
-
-_EAGER = "warp_route.eager_graph"  # metadata key of a leaf's gradient accumulator
-
-
-def _accumulators(tensors):
-    """Metadata of the leaves' gradient accumulators, which live as long as a
-    graph that uses them."""
-    for t in tensors:
-        if t.requires_grad and t.is_leaf:
-            yield torch.autograd.graph.get_gradient_edge(t).node.metadata
-
-
-def _differentiable_ffn(leaves, *args: torch.Tensor) -> torch.Tensor:
-    """_GatedFFN, refused under graph capture while an eager graph of the leaves
-    among ``leaves`` is alive.  Their gradient accumulators then belong to the eager
-    graph's stream, for which the captured backward pass would wait; torch does
-    not survive that.  Eager calls mark the accumulators, captured ones look
-    for the mark."""
-    if not args[0].is_cuda or not torch.cuda.is_current_stream_capturing():
-        y = _GatedFFN.apply(*args)
-        for mark in _accumulators(leaves):
-            mark[_EAGER] = True
-        return y
-    if any(_EAGER in mark for mark in _accumulators(leaves)):
-        raise RuntimeError("gated_ffn is captured into a graph while an eager autograd graph of "
-                           "the same tensors is alive: drop its outputs before the capture")
-    return _GatedFFN.apply(*args)
-
-
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x [..., n] as [rows, n]."""
     if x.dim() == 0:
@@ -461,17 +415,11 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     arguments; gradients that are not needed are not computed.
 
     Forward and backward launch kernels on the current stream only and may be
-    captured in a HIP graph.  When a backward pass is captured, no eager graph
-    of the same leaf tensors may be alive (as for any torch operator); one
-    that a call of this function made raises RuntimeError.
+    captured in a HIP graph.  While a differentiable call is captured, no eager
+    autograd graph of the same leaf tensors may be alive, which raises
+    RuntimeError: the captured backward pass would wait for that graph's stream.
     """
-    rows = _rows(x)
-    leaves = (x, w_gate, w_up, w_down)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in leaves):
-        y = _differentiable_ffn(leaves, rows, w_gate, w_up, w_down)
-    else:
-        y = _load_extension().gated_ffn_forward(rows, w_gate, w_up, w_down, False)[0]
-    return y if x.dim() == 2 else y.reshape(x.shape)
+    return _load_extension().gated_ffn(x, w_gate, w_up, w_down)
 
 
 def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
