@@ -453,3 +453,71 @@ def test_modules_and_stack(cuda):
             assert torch.equal(step(rows), want)
             stack(rows)
         assert torch.equal(MoEStack(layers, E, h, I, k, shared=[None, None])(rows), plain(rows))
+
+
+@pytest.mark.parametrize("T,h,I", [(3, 50, 75), (40, 33, 129), (257, 130, 71)])
+def test_c_abi_writes_its_outputs_only(cuda, T, h, I):
+    """Direct calls of the C-ABI with a canary behind every buffer it writes,
+    the workspace of exactly the size asked for."""
+    import ctypes
+    from warp_route import capi
+    lib, guard = capi.lib(), 4096
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    x, *w = layer(T, h, I, torch.float16, cuda)
+    dy = tokens(9, T, h, torch.float16, cuda)
+    kept = []
+
+    def buffer(nbytes):
+        t = torch.full((nbytes + guard,), 0xA5, dtype=torch.uint8, device=cuda)
+        kept.append((t, nbytes))
+        return t
+
+    row = lib.wr_ffn_saved_row(I)
+    a = capi.WrFfnArgs()
+    a.dtype, a.batch_size, a.hidden_dim, a.intermediate_dim = capi.WR_F16, T, h, I
+    for name, t in zip(("x", "w_gate", "w_up", "w_down", "dout"), (x, *w, dy)):
+        setattr(a, name, t.data_ptr())
+    bufs = {n: buffer(b) for n, b in (
+        ("out", 2 * T * h), ("saved_gate", 4 * T * row), ("saved_up", 4 * T * row),
+        ("saved_act", 2 * T * row), ("dx", 2 * T * h), ("dw_gate", 2 * I * h), ("dw_up", 2 * I * h),
+        ("dw_down", 2 * I * h))}
+    for n, t in bufs.items():
+        setattr(a, n, t.data_ptr())
+    for entry, back in (("wr_ffn_forward", 0), ("wr_ffn_backward", 1)):
+        a.workspace_bytes = lib.wr_ffn_workspace_bytes(back, a.dtype, h, I, T)
+        a.workspace = buffer(a.workspace_bytes).data_ptr()
+        assert getattr(lib, entry)(ctypes.byref(a), stream) == capi.WR_OK
+
+    def shaped(n, r, c):
+        return bufs[n][:2 * r * c].view(torch.float16).view(r, c)
+
+    torch.cuda.synchronize()
+    O.assert_within(shaped("out", T, h), *O.ffn(x, *w), "y")
+    shapes = {"dx": (T, h), "dw_gate": (I, h), "dw_up": (I, h), "dw_down": (h, I)}
+    for (n, s), ref in zip(shapes.items(), O.ffn_grads(x, *w, dy)):
+        O.assert_within(shaped(n, *s), *ref, n)
+
+    (q, sx), (p, sp), (d, sd) = (F.quantize_int8(t) for t in w)
+    m = capi.WrFfnInt8Args()
+    m.dtype, m.batch_size, m.hidden_dim, m.intermediate_dim = capi.WR_F16, T, h, I
+    for name, t in zip(("x", "w_gate", "s_gate", "w_up", "s_up", "w_down", "s_down"),
+                       (x, q, sx, p, sp, d, sd)):
+        setattr(m, name, t.data_ptr())
+    m.out = buffer(2 * T * h).data_ptr()
+    m.workspace_bytes = lib.wr_ffn_int8_workspace_bytes(h, I, T)
+    m.workspace = buffer(m.workspace_bytes).data_ptr()
+    assert lib.wr_ffn_int8(ctypes.byref(m), stream) == capi.WR_OK
+    codes, scales = buffer(T * h), buffer(4 * T)
+    assert lib.wr_quantize_int8(x.data_ptr(), capi.WR_F16, T, h, codes.data_ptr(),
+                                scales.data_ptr(), stream) == capi.WR_OK
+    k = capi.WrInt8Args()
+    k.out_dtype, k.rows, k.out_features, k.in_features = capi.WR_F32, T, I, h
+    for name, t in zip(("x", "x_scale", "w", "w_scale"), (codes, scales, q, sx)):
+        setattr(k, name, t.data_ptr())
+    k.out = buffer(4 * T * I).data_ptr()
+    k.workspace_bytes = lib.wr_int8_workspace_bytes(T, I, h)
+    k.workspace = buffer(k.workspace_bytes).data_ptr()
+    assert lib.wr_int8_matmul(ctypes.byref(k), stream) == capi.WR_OK
+    torch.cuda.synchronize()
+    for t, n in kept:
+        assert (t[n:] == 0xA5).all()

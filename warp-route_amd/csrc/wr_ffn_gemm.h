@@ -117,12 +117,6 @@ struct TileCopy {
   static constexpr int EPC = 16 / ES;  // elements per chunk
   unsigned voff[PER];
 
-  // Chunk of this lane in copy j, as a k offset (KC).
-  static __device__ __forceinline__ int k_chunk(int j, int wave, int lane) {
-    const int row = (j * NW + wave) * 8 + (lane >> 3);
-    return (lane & 7) ^ kc_key<NSIDE>(row);
-  }
-
   // left: elements left from the tile's first one, of m (n) (KS) or of K (KC: KB or more
   // except at the last step of a segment).
   __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int left) {
