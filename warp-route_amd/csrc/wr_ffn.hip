@@ -253,17 +253,19 @@ hipError_t launch_zero(void* p, int64_t bytes, hipStream_t s) {
 struct ShapeCost {
   int bm, bn, per_cu;  // tile, blocks a CU holds
   float step;          // us per 128 bytes of K, with per_cu blocks on the CU
-  float alone;         // the same with one
+  float alone;         // the same where a round leaves CUs free, or one block on each
   float fixed;         // us per tile: first copies, epilogue
 };
 // Measured on one MI355X (bf16; 16 times the clocks for fp32).  Tiles of 128 x 128 with 3
 // buffers against 2: 64 x 4096 by 4096 x 14336 (112 tiles) 31 against 41 us, 4096 x
 // 2816 by 2816 x 2048 (512 tiles) 55 against 44; against 256 x 256 at 2048 x 4096 by
 // 4096 x 14336 207 and 183 us.  64 x 256 tiles were slower than 128 x 128 throughout.
-constexpr ShapeCost kCost16[kShapes] = {
-    {256, 256, 1, 1.37f, 1.37f, 5.0f}, {128, 128, 2, 0.92f, 0.58f, 3.0f}, {128, 128, 1, 0.45f, 0.45f, 3.0f}};
-constexpr ShapeCost kCost32[kShapes] = {
-    {256, 256, 1, 7.7f, 7.7f, 6.0f}, {128, 128, 2, 4.0f, 2.2f, 4.0f}, {128, 128, 1, 2.2f, 2.2f, 4.0f}};
+constexpr ShapeCost kCost16[kShapes] = {{256, 256, 1, 1.37f, 1.37f, 5.0f},
+                                        {128, 128, 2, 0.92f, 0.58f, 3.0f},
+                                        {128, 128, 1, 0.55f, 0.45f, 3.0f}};
+constexpr ShapeCost kCost32[kShapes] = {{256, 256, 1, 7.7f, 7.7f, 6.0f},
+                                        {128, 128, 2, 4.0f, 2.2f, 4.0f},
+                                        {128, 128, 1, 2.2f, 2.2f, 4.0f}};
 constexpr int kCUs = 256;
 constexpr int kMaxSlices = 32;
 constexpr int64_t kMaxPartBytes = (int64_t)512 << 20;
@@ -273,12 +275,12 @@ struct Plan {
   size_t part_bytes;
 };
 
-// epi: bytes that the epilogue reads and writes per element of the tile.  A CU moves about
-// 20 KB a us; two blocks on a CU hide half of it behind each other's products.
+// epi: bytes that the epilogue reads and writes per element of the tile; a CU moves about
+// 20 KB a us.
 float rounds_us(const ShapeCost& c, int64_t blocks, int steps, float epi) {
   const int64_t cap = (int64_t)kCUs * c.per_cu, rest = blocks % cap;
   const float move = epi * c.bm * c.bn / 20e3f;
-  const float full = steps * c.step + c.fixed + move;
+  const float full = steps * c.step + c.fixed + move * c.per_cu;
   return blocks / cap * full +
          (rest == 0 ? 0.0f : rest <= kCUs ? steps * c.alone + c.fixed + move : full);
 }
@@ -314,11 +316,14 @@ Plan plan_of(int M, int N, int K, int es, int nseg, int nprob, bool gated, float
       const int64_t whole = S == 1 ? tiles : tiles - rest;
       const int64_t part = (tiles - whole) * S * c.bm * c.bn * 4;
       if (S > 1 && (rest == 0 || part > kMaxPartBytes)) break;
-      // The join reads them (they are written like an epilogue); not those of rows past M.
-      const float moved = part * std::min(1.0f, (float)M / (tm * c.bm));
+      // The slices' sums are written like an epilogue; the join reads them (not those of rows
+      // past M) and has the tiles' own epilogue.
+      const float moved = (part + (tiles - whole) * c.bm * c.bn * epi) *
+                          std::min(1.0f, (float)M / (tm * c.bm));
       const float us = rounds_us(c, whole, steps, epi) +
                        (S == 1 ? 0.0f
-                               : rounds_us(c, rest * S, (steps + S - 1) / S, 4.0f) + 4.0f + moved / 4e6f);
+                               : rounds_us(c, rest * S, (steps + S - 1) / S, 4.0f) + 4.0f +
+                                     moved / 5e6f);
       if (best.tiles == 0 || us < best_us) {
         best = {shape, S, (int)tm, (int)tn, (int)tiles, (int)whole, (size_t)part};
         best_us = us;
