@@ -259,7 +259,8 @@ struct ShapeCost {
 // Measured on one MI355X (bf16; 16 times the clocks for fp32).  Tiles of 128 x 128 with 3
 // buffers against 2: 64 x 4096 by 4096 x 14336 (112 tiles) 31 against 41 us, 4096 x
 // 2816 by 2816 x 2048 (512 tiles) 55 against 44; against 256 x 256 at 2048 x 4096 by
-// 4096 x 14336 207 and 183 us.  64 x 256 tiles were slower than 128 x 128 throughout.
+// 4096 x 14336 207 and 183 us.  64 x 256 tiles were slower than the better 128 x 128 at
+// every size measured.
 constexpr ShapeCost kCost16[kShapes] = {{256, 256, 1, 1.37f, 1.37f, 5.0f},
                                         {128, 128, 2, 0.92f, 0.58f, 3.0f},
                                         {128, 128, 1, 0.55f, 0.45f, 3.0f}};

@@ -1,9 +1,10 @@
-"""ctypes binding of the C-ABI in include/warp_route.h (libwarp_route_hip.so).
+"""ctypes binding of the C-ABI in include/warp_route.h and include/wr_ffn.h
+(libwarp_route_hip.so).
 
 This is the binding a caller without the torch extension uses: plain device
-pointers, sizes and a hipStream_t passed as an integer.  It mirrors the header
-field for field; ``tests/test_abi.py`` checks that every declared entry point
-is exported.
+pointers, sizes and a hipStream_t passed as an integer.  It mirrors the headers
+field for field; ``tests/test_abi.py`` and ``tests/test_ffn_host.py`` check that
+every declared entry point is exported.
 """
 from __future__ import annotations
 
