@@ -30,6 +30,9 @@ extern "C" {
 
 /* Largest hidden_dim, intermediate_dim, and rows or columns of a weight. */
 #define WR_FFN_MAX_DIM (1 << 20)
+/* Most rows (tokens) of a call, and most columns that wr_quantize_int8 takes. */
+#define WR_FFN_MAX_ROWS (1 << 28)
+#define WR_INT8_MAX_COLS (1 << 30)
 /* Largest K of an int8 product: 128 * 128 * K stays inside an int32. */
 #define WR_INT8_MAX_K 131071
 

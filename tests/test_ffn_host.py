@@ -148,6 +148,33 @@ def test_int8_validation():
     assert "16-byte" in capi.status_str(capi.WR_EINVAL_ALIGN)
 
 
+@pytest.mark.parametrize("n", [(1 << 28) + 1, (1 << 31) - 1])
+def test_more_rows_than_the_grid_is_planned_for_are_refused(n):
+    """Rows are rounded up to tiles in 32 bits: 2**31 - 1 of them would wrap."""
+    lib = capi.lib()
+    assert n > capi.WR_FFN_MAX_ROWS
+    a = capi.WrFfnArgs()
+    for name, _ in capi.WrFfnArgs._fields_[:13]:
+        setattr(a, name, FAKE)
+    a.dtype, a.batch_size, a.hidden_dim, a.intermediate_dim = capi.WR_F16, n, 1, 1
+    a.workspace, a.workspace_bytes = FAKE, 1 << 60
+    assert lib.wr_ffn_forward(ctypes.byref(a), None) == capi.WR_EINVAL_BATCH
+    assert lib.wr_ffn_backward(ctypes.byref(a), None) == capi.WR_EINVAL_BATCH
+    assert lib.wr_ffn_workspace_bytes(0, capi.WR_F16, 1, 1, n) == 0
+    assert lib.wr_int8_workspace_bytes(n, 1, 1) == 0
+    assert lib.wr_ffn_int8_workspace_bytes(1, 1, n) == 0
+    assert lib.wr_int8_workspace_bytes(capi.WR_FFN_MAX_ROWS, 1, 1) >= 16 * capi.WR_FFN_MAX_ROWS
+    assert lib.wr_quantize_int8(FAKE, capi.WR_F16, n, 8, FAKE, FAKE, None) == capi.WR_EINVAL_BATCH
+
+
+@pytest.mark.parametrize("cols", [(1 << 30) + 1, (1 << 31) - 1])
+def test_columns_past_the_row_loop_are_refused(cols):
+    """A step past the last column has to fit 32 bits, or the loop would not end."""
+    assert cols > capi.WR_INT8_MAX_COLS
+    st = capi.lib().wr_quantize_int8(FAKE, capi.WR_F16, 1, cols, FAKE, FAKE, None)
+    assert st == capi.WR_EINVAL_SHAPE
+
+
 def test_python_entry_points_refuse_host_tensors():
     x, w = torch.zeros(2, 8), torch.zeros(4, 8)
     for call in (lambda: F.gated_ffn(x, w, w, w.t().contiguous()), lambda: F.quantize_int8(x),

@@ -320,7 +320,7 @@ void check_tokens(const torch::Tensor& x, const char* name) {
   TORCH_CHECK(x.is_cuda(), name, " must be a CUDA (HIP) tensor");
   TORCH_CHECK(x.is_contiguous(), name, " must be contiguous");
   TORCH_CHECK(x.dim() == 2, name, " must have shape [rows, columns], got shape ", x.sizes());
-  TORCH_CHECK(x.size(0) <= INT32_MAX && x.size(1) >= 1, name, " has an unsupported shape ",
+  TORCH_CHECK(x.size(0) <= WR_FFN_MAX_ROWS && x.size(1) >= 1, name, " has an unsupported shape ",
               x.sizes());
 }
 
@@ -534,7 +534,7 @@ torch::Tensor gated_ffn(const torch::Tensor& x, const torch::Tensor& w_gate,
 std::tuple<torch::Tensor, torch::Tensor> quantize_int8(torch::Tensor x) {
   check_tokens(x, "x");
   const int tag = float_tag(x, "x");
-  TORCH_CHECK(x.size(1) <= INT32_MAX, "x has an unsupported shape ", x.sizes());
+  TORCH_CHECK(x.size(1) <= WR_INT8_MAX_COLS, "x has an unsupported shape ", x.sizes());
   const torch::Device dev = x.device();
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   x = aligned16(x);

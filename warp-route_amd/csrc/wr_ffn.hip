@@ -571,7 +571,7 @@ int check_ffn(const wr_ffn_args* a) {
   if (a->hidden_dim < 1 || a->intermediate_dim < 1 || a->hidden_dim > WR_FFN_MAX_DIM ||
       a->intermediate_dim > WR_FFN_MAX_DIM)
     return WR_EINVAL_SHAPE;
-  if (a->batch_size < 0) return WR_EINVAL_BATCH;
+  if (a->batch_size < 0 || a->batch_size > WR_FFN_MAX_ROWS) return WR_EINVAL_BATCH;
   for (const void* p : {a->x, a->w_gate, a->w_up, a->w_down, (const void*)a->workspace,
                         (const void*)a->saved_gate, (const void*)a->saved_up,
                         (const void*)a->saved_act})
@@ -648,8 +648,8 @@ int wr_ffn_backward(const wr_ffn_args* a, void* stream) {
 int wr_quantize_int8(const void* x, int dtype, int rows, int cols, int8_t* codes, float* scales,
                      void* stream) {
   if (!float_dtype(dtype)) return WR_EINVAL_DTYPE;
-  if (rows < 0) return WR_EINVAL_BATCH;
-  if (cols < 1) return WR_EINVAL_SHAPE;
+  if (rows < 0 || rows > WR_FFN_MAX_ROWS) return WR_EINVAL_BATCH;
+  if (cols < 1 || cols > WR_INT8_MAX_COLS) return WR_EINVAL_SHAPE;
   if (rows == 0) return WR_OK;
   if (!x || !codes || !scales) return WR_EINVAL_NULL;
   if (!aligned(x) || !aligned(codes) || !aligned(scales)) return WR_EINVAL_ALIGN;
@@ -665,7 +665,7 @@ static int check_int8(const wr_int8_args* a) {
   if (a->out_features < 1 || a->in_features < 1 || a->out_features > WR_FFN_MAX_DIM ||
       a->in_features > WR_INT8_MAX_K)
     return WR_EINVAL_SHAPE;
-  if (a->rows < 0) return WR_EINVAL_BATCH;
+  if (a->rows < 0 || a->rows > WR_FFN_MAX_ROWS) return WR_EINVAL_BATCH;
   return WR_OK;
 }
 
@@ -695,7 +695,7 @@ static int check_ffn_int8(const wr_ffn_int8_args* a) {
   if (a->hidden_dim < 1 || a->intermediate_dim < 1 || a->hidden_dim > WR_INT8_MAX_K ||
       a->intermediate_dim > WR_INT8_MAX_K)
     return WR_EINVAL_SHAPE;
-  if (a->batch_size < 0) return WR_EINVAL_BATCH;
+  if (a->batch_size < 0 || a->batch_size > WR_FFN_MAX_ROWS) return WR_EINVAL_BATCH;
   return WR_OK;
 }
 

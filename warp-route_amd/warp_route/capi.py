@@ -48,6 +48,8 @@ WR_KIND_NAIVE = 2
 # include/wr_ffn.h
 WR_FFN_MAX_DIM = 1 << 20
 WR_INT8_MAX_K = 131071
+WR_FFN_MAX_ROWS = 1 << 28
+WR_INT8_MAX_COLS = 1 << 30
 
 
 class WrOffsets(ctypes.Structure):

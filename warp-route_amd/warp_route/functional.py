@@ -403,7 +403,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     """Dense gated FFN: (silu(x w_gate^T) * (x w_up^T)) w_down^T.
 
     Args:
-        x: tokens [..., hidden_dim], any number of them, float32, float16 or
+        x: tokens [..., hidden_dim], up to 2**28 of them, float32, float16 or
             bfloat16, contiguous, on the GPU.
         w_gate, w_up: [intermediate_dim, hidden_dim] in x's dtype.
         w_down: [hidden_dim, intermediate_dim] in x's dtype.
@@ -411,8 +411,9 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     Returns x's shape and dtype.  Sums are fp32; the activations between the
     two products are rounded to x's dtype.  When a gradient is needed, three
     buffers of x's rows times intermediate_dim are kept for it: both
-    pre-activations in fp32 and the activations in x's dtype.  Differentiable once with respect to all four
-    arguments; gradients that are not needed are not computed.
+    pre-activations in fp32 and the activations in x's dtype.  Differentiable
+    once with respect to all four arguments; gradients that are not needed are
+    not computed.
 
     Forward and backward launch kernels on the current stream only and may be
     captured in a HIP graph.  While a differentiable call is captured, no eager
@@ -428,7 +429,7 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     max|row| rounded to nearest, ties to even, exactly.  A zero row gets codes
     0 and scale 1; a row with a non-finite value gets codes 0 and scale NaN, so
     that only what is computed from it is NaN.  Codes have x's shape, scales
-    x's shape without its last dimension."""
+    x's shape without its last dimension.  Up to 2**28 rows of 2**30 columns."""
     q, s = _load_extension().quantize_int8(_rows(x))
     return q.reshape(x.shape), s.reshape(x.shape[:-1])
 
