@@ -239,6 +239,17 @@ def test_quantize_extremes(cuda, dtype):
     O.assert_within(s, ws, 1.01 * O.E * ws + O.step(torch.float32), "scales")
 
 
+def test_quantize_more_rows_than_one_launch_holds(cuda):
+    """2^26 rows of 64 threads are 2^32 threads, more than a launch holds.  One column:
+    codes are the sign times 127, 0 for a zero, which any row can be held against."""
+    rows = (1 << 26) + 5
+    x = torch.arange(rows, device=cuda, dtype=torch.int32).remainder_(3).sub_(1).to(torch.float16)
+    q, s = F.quantize_int8(x.view(rows, 1))
+    assert torch.equal(q.view(-1), x.to(torch.int8) * 127)
+    one = torch.tensor(1.0 / 127.0, device=cuda)  # 1 / 127 rounded to fp32, as a division is
+    assert torch.equal(s, torch.where(x == 0, torch.ones_like(one), one))
+
+
 def test_same_bits_every_time(cuda):
     for T, h, I in [(1, 512, 256), (16, 4096, 1024), (48, 515, 515), (65, 512, 4096), (700, 512, 520)]:
         args = layer(T, h, I, torch.float16, cuda)

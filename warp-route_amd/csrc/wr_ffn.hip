@@ -197,11 +197,21 @@ hipError_t launch_quantize_as(const T* x, int rows, int cols, int8_t* codes, int
   // Two vectors a thread: their latency overlaps, and short rows take few waves.
   constexpr int per = 2 * 16 / sizeof(T);
   const int threads = std::min(1024, std::max(64, (cols + per * 64 - 1) / (per * 64) * 64));
-  if (cols % (per / 2) == 0)
-    k_quantize<T, true><<<rows, threads, 0, s>>>(x, cols, codes, ldc, scales, zero_max);
-  else
-    k_quantize<T, false><<<rows, threads, 0, s>>>(x, cols, codes, ldc, scales, zero_max);
-  return hipGetLastError();
+  // A launch holds fewer than 2^32 threads: 2^21 rows of 1024.
+  constexpr int most = 1 << 21;
+  for (int64_t at = 0; at < rows; at += most) {
+    const int n = (int)std::min<int64_t>(most, rows - at);
+    unsigned* const zero = zero_max == nullptr ? nullptr : zero_max + at;
+    if (cols % (per / 2) == 0)
+      k_quantize<T, true>
+          <<<n, threads, 0, s>>>(x + at * cols, cols, codes + at * ldc, ldc, scales + at, zero);
+    else
+      k_quantize<T, false>
+          <<<n, threads, 0, s>>>(x + at * cols, cols, codes + at * ldc, ldc, scales + at, zero);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_quantize(const void* x, int dtype, int rows, int cols, int8_t* codes, int64_t ldc,
